@@ -1,0 +1,369 @@
+"""Cases of the 4-bit K/V cache operators: storing rows, reading them back, attention over them.
+
+A cache holds, per (slot, kv head), blocks of 64 tokens of 4608 bytes:
+    K codes [64][32] | K (c, d) [64][2] f16 | V codes [64][32] | V (c, d) [64][2] f16
+A group is the 64 elements of one token and kv head: element i has the nibble n' + 8 (low
+nibble of byte i / 2 when i is even) and the value c + d n'.  With `own` false the operators
+run in their plain form on the same bytes; with `own` true through madi_b200.kv4.
+"""
+import math
+
+import torch
+
+own = False
+
+HD = 64               # head_dim
+BLK = 64              # tokens per block
+ROW = 36              # bytes a group takes: 32 of codes, 4 of (c, d)
+BLOCK_BYTES = 2 * BLK * ROW
+LIMIT = 57344.0       # larger magnitudes make the group NaN
+DT = {"f32": torch.float32, "f16": torch.float16}
+
+
+# ----------------------------------------------------------------------------- cases
+
+def listed():
+    return [
+        # the append of a greedy token step: one new f32 row per head, one slot, a 448-row self cache
+        dict(name="store_token_1", op="store", slots=1, T=1, kv_heads=20, max_tok=448, dtype="f32", ragged=False),
+        # the cross K/V of 8 audio chunks: all 1500 encoder positions at once, f16
+        dict(name="store_chunks_8", op="store", slots=8, T=1500, kv_heads=20, max_tok=1500, dtype="f16", ragged=False),
+        # a ragged batch of long prompts behind rows already cached, grouped heads
+        dict(name="store_prompts_4", op="store", slots=4, T=9001, kv_heads=8, max_tok=20000, dtype="f16", ragged=True),
+        # one chunk's cross cache read back as f16 (e.g. for the scores of the f16 attention)
+        dict(name="load_chunk_1", op="load", slots=1, T=1500, kv_heads=20, max_tok=1500, dtype="f16", ragged=False),
+        # long cached contexts read back as f32
+        dict(name="load_long_2", op="load", slots=2, T=30011, kv_heads=8, max_tok=32768, dtype="f32", ragged=True),
+        # a token step's self-attention, one slot: latency
+        dict(name="token_self_1", op="attn", slots=1, T=1, heads=20, kv_heads=20, max_tok=448, mode="pos",
+             dtype="f32", ragged=False),
+        # a token step's cross-attention at 8 slots: the step's largest read
+        dict(name="token_cross_8", op="attn", slots=8, T=1, heads=20, kv_heads=20, max_tok=1500, mode="all",
+             dtype="f32", ragged=False),
+        # a padded batch of 16 slots with lengths from 0 up, self cache
+        dict(name="token_ragged_16", op="attn", slots=16, T=1, heads=20, kv_heads=20, max_tok=448, mode="lens",
+             dtype="f32", ragged=True),
+        # serving over long contexts, four query heads to a kv head, f16
+        dict(name="token_long_4", op="attn", slots=4, T=1, heads=32, kv_heads=8, max_tok=65003, mode="lens",
+             dtype="f16", ragged=True),
+        # five draft tokens per slot checked against the model in one step
+        dict(name="draft_8", op="attn", slots=8, T=5, heads=20, kv_heads=20, max_tok=448, mode="pos", dtype="f32",
+             ragged=True),
+        # prompts of 224 tokens (half the decoder's context) over 8 chunks' cross caches
+        dict(name="prompt_cross_8", op="attn", slots=8, T=224, heads=20, kv_heads=20, max_tok=1500, mode="all",
+             dtype="f16", ragged=False),
+        # a chunk of a long prompt attending to itself and to what is cached before it
+        dict(name="prompt_long_2", op="attn", slots=2, T=1024, heads=32, kv_heads=8, max_tok=16640, mode="pos",
+             dtype="f16", ragged=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    most_b = max(work(c)["bytes"] for c in listed())
+    most_f = max(work(c)["flops"] for c in listed())
+    while True:
+        op = rng.choice(("store", "load", "attn", "attn", "attn"))
+        slots, kvh = _log(rng, 1, 16), rng.choice((1, 2, 4, 5, 6, 8, 12, 20))
+        dtype, ragged = rng.choice(("f32", "f16")), rng.random() < 0.5
+        if op != "attn":
+            T = _log(rng, 1, 30000)
+            c = dict(op=op, slots=slots, T=T, kv_heads=kvh, max_tok=T + _log(rng, 1, 3000), dtype=dtype, ragged=ragged)
+        else:
+            group = rng.choice((1, 1, 2, 3, 4, 8))
+            T = rng.choice((1, 1, _log(rng, 2, 16), _log(rng, 16, 1200)))
+            if T > 64:
+                dtype = "f16"
+            c = dict(op=op, slots=slots, T=T, heads=kvh * group, kv_heads=kvh, max_tok=T + _log(rng, 1, 60000),
+                     mode=rng.choice(("pos", "lens", "all")), dtype=dtype, ragged=ragged)
+            # what a plain pass holds: its scores and the cache in 32 bits
+            if c["slots"] * c["heads"] * c["T"] * c["max_tok"] > 1.1e9 or slots * kvh * c["max_tok"] > 3e6:
+                continue
+        w = work(c)
+        if w["bytes"] <= most_b and w["flops"] <= most_f:
+            return c
+
+
+def _counts(case):
+    """(first row or key count per slot, valid rows per slot): the batch's lengths, which belong to the case."""
+    S, T, M = case["slots"], case["T"], case["max_tok"]
+    part = [(S - s) / S for s in range(S)] if case["ragged"] else [1.0] * S
+    n = [max(1, int(T * p)) if T > 1 else 1 for p in part]
+    if case["op"] == "attn" and case["mode"] == "lens":
+        first = [int(M * p) for p in part]
+        if case["ragged"] and S > 2:
+            first[-1] = 0                                   # an empty slot
+    elif case["op"] == "load":
+        first = [0] * S
+    else:
+        first = [int((M - T) * p) for p in part]            # rows cached before the new ones
+    return first, n
+
+
+def _keys(case):
+    """How many keys each valid query of each slot attends to."""
+    first, n = _counts(case)
+    M = case["max_tok"]
+    if case["mode"] == "pos":
+        return [[min(f + i + 1, M) for i in range(k)] for f, k in zip(first, n)]
+    return [[min(f, M) if case["mode"] == "lens" else M] * k for f, k in zip(first, n)]
+
+
+def work(case):
+    H, (first, n) = case["kv_heads"], _counts(case)
+    e = 4 if case["dtype"] == "f32" else 2
+    if case["op"] == "store":                                # rows in, codes out, codes in, rows out (f32)
+        r = 2 * sum(n) * H
+        return {"bytes": r * (HD * e + 2 * ROW + HD * 4), "flops": r * HD * 6}
+    if case["op"] == "load":
+        r = 2 * sum(n) * H
+        return {"bytes": r * (ROW + HD * e), "flops": r * HD * 2}
+    k = _keys(case)
+    return {"bytes": sum(max(r) for r in k) * H * 2 * ROW + 2 * sum(n) * case["heads"] * HD * e,
+            "flops": 4 * HD * case["heads"] * sum(sum(r) for r in k)}
+
+
+# ----------------------------------------------------------------------------- inputs
+
+def _u32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    S, T, H, M = case["slots"], case["T"], case["kv_heads"], case["max_tok"]
+    dt = DT[case["dtype"]]
+    first, n = _counts(case)
+    nb = (M + BLK - 1) // BLK
+    st = dict(case=case, max_tok=M, data=torch.full((S, H, nb, BLOCK_BYTES), 0xFF, dtype=torch.uint8, device="cuda"))
+    ragged_n = T > 1 and case["ragged"]
+    st["n"] = _u32(n) if ragged_n else None
+    if case["op"] == "store":
+        # keys with an offset per channel, as decoder keys have; values around zero
+        off = torch.randn((1, 1, H * HD), generator=g, device="cuda")
+        st["k"] = (torch.randn((S, T, H * HD), generator=g, device="cuda") + off).to(dt)
+        st["v"] = (0.5 * torch.randn((S, T, H * HD), generator=g, device="cuda")).to(dt)
+        st["pos"] = _u32(first)
+        st["k_out"] = torch.zeros((S, T, H * HD), dtype=torch.float32, device="cuda")
+        st["v_out"] = torch.zeros_like(st["k_out"])
+        return st
+    # a written cache: bell-shaped codes, steps of 8 significant bits; rows that no slot has
+    # reached keep 0xFF bytes, whose (c, d) are NaN
+    rows = torch.arange(nb * BLK, device="cuda").view(1, 1, nb, BLK, 1)
+    if case["op"] == "load":
+        top = n
+    elif case["mode"] == "pos":
+        top = [f + k for f, k in zip(first, n)]
+    else:
+        top = first if case["mode"] == "lens" else [M] * S
+    there = rows < _u32(top).view(S, 1, 1, 1, 1)
+    for at, spread in ((0, 1.0), (BLK * ROW, 0.5)):
+        codes = st["data"][..., at:at + BLK * 32].unflatten(-1, (BLK, 32))
+        z = torch.randn((S, H, nb, BLK, HD), generator=g, device="cuda", dtype=torch.float16)
+        z = z.mul_(3.2).add_(8.5).clamp_(0, 15).to(torch.uint8)
+        codes.copy_(torch.where(there, z[..., 0::2] | (z[..., 1::2] << 4), codes))
+        cd = torch.randn((S, H, nb, BLK, 2), generator=g, device="cuda", dtype=torch.float32)
+        cd[..., 0].mul_(0.2 * spread)
+        cd[..., 1] = ((0.3 + 0.04 * cd[..., 1]).clamp_(min=0.05) * spread).to(torch.bfloat16).float()
+        par = st["data"][..., at + BLK * 32:at + BLK * ROW].unflatten(-1, (BLK, 4))
+        par.copy_(torch.where(there, cd.to(torch.float16).view(torch.uint8), par))
+    if case["op"] == "load":
+        st["k_out"] = torch.zeros((S, T, H * HD), dtype=dt, device="cuda")
+        st["v_out"] = torch.zeros_like(st["k_out"])
+        return st
+    st["q"] = torch.randn((S, T, case["heads"] * HD), generator=g, device="cuda").mul_(1.5).to(dt)
+    st["out"] = torch.zeros_like(st["q"])
+    st["pos"] = _u32(first) if case["mode"] == "pos" else None
+    st["lens"] = _u32(first) if case["mode"] == "lens" else None
+    return st
+
+
+# ----------------------------------------------------------------------------- one pass
+
+def run(st):
+    case = st["case"]
+    if own:
+        from madi_b200 import kv4
+        cache = kv4.Cache(st["data"], st["max_tok"])
+        if case["op"] == "store":
+            kv4.store(cache, st["k"], st["v"], pos=st["pos"], n=st["n"])
+            return kv4.load(cache, case["T"], pos=st["pos"], n=st["n"], k_out=st["k_out"], v_out=st["v_out"])
+        if case["op"] == "load":
+            return kv4.load(cache, case["T"], n=st["n"], k_out=st["k_out"], v_out=st["v_out"])
+        return kv4.attn(st["q"], cache, case["heads"], pos=st["pos"], lens=st["lens"], n=st["n"], out=st["out"])
+    if case["op"] == "store":
+        _plain_store(st)
+        return _plain_load(st, st["pos"])
+    if case["op"] == "load":
+        return _plain_load(st, torch.zeros(case["slots"], dtype=torch.int32, device="cuda"))
+    return _plain_attn(st)
+
+
+def _parts(st, at):
+    """Codes [S][H][blocks][64][32] and (c, d) bytes [S][H][blocks][64][4] of K (at 0) or V: views."""
+    d = st["data"]
+    return (d[..., at:at + BLK * 32].unflatten(-1, (BLK, 32)), d[..., at + BLK * 32:at + BLK * ROW].unflatten(-1, (BLK, 4)))
+
+
+def _rows(st, pos):
+    """Cache row of each new row [S][T], and whether it is one (not padding, inside the cache)."""
+    case = st["case"]
+    i = torch.arange(case["T"], device="cuda").view(1, -1)
+    r = pos.long().view(-1, 1) + i
+    ok = r < st["max_tok"]
+    if st["n"] is not None:
+        ok = ok & (i < st["n"].long().view(-1, 1))
+    return r, ok
+
+
+def _quantise(x):
+    """x [..., 64] -> (codes [..., 32] u8, (c, d) [..., 2] f16): ranges next to a border need 64 bits."""
+    x = x.float()
+    lo, hi = x.amin(-1), x.amax(-1)
+    bad = ~(x.abs() <= LIMIT).all(-1)
+    c = (lo + (hi - lo) * torch.tensor(8 / 15, dtype=torch.float32, device=x.device)).half()
+    x, lo, hi, c64 = x.double(), lo.double(), hi.double(), c.double()
+    r = torch.maximum((c64 - lo) / 8, (hi - c64) / 7)
+    _, e = torch.frexp(r)
+    step = torch.ldexp(torch.ones_like(r), (e - 8).clamp(min=-24))
+    d = torch.ceil(r / step) * step
+    ok = (d > 0) & ~bad
+    nq = torch.floor((x - c64.unsqueeze(-1)) / torch.where(ok, d, 1.0).unsqueeze(-1) + 0.5)
+    z = (torch.where(ok.unsqueeze(-1), nq, 0.0) + 8).to(torch.uint8)
+    cd = torch.stack((torch.where(bad, float("nan"), c64), torch.where(bad, 0.0, d)), -1).half()
+    return z[..., 0::2] | (z[..., 1::2] << 4), cd
+
+
+def _plain_store(st):
+    case = st["case"]
+    r, ok = _rows(st, st["pos"])
+    s = torch.arange(case["slots"], device="cuda").view(-1, 1).expand_as(r)[ok]
+    blk, off = r[ok] // BLK, r[ok] % BLK
+    for x, at in ((st["k"], 0), (st["v"], BLK * ROW)):
+        codes, cd = _quantise(x[ok].unflatten(-1, (case["kv_heads"], HD)))         # [rows][H][..]
+        to_codes, to_cd = _parts(st, at)
+        to_codes.permute(0, 2, 3, 1, 4)[s, blk, off] = codes
+        to_cd.permute(0, 2, 3, 1, 4)[s, blk, off] = cd.view(torch.uint8)
+
+
+def _values(codes, par):
+    """f32 values [..., 64] of codes [..., 32] and (c, d) bytes [..., 4]."""
+    cd = par.contiguous().view(torch.float16).float()
+    z = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).float() - 8
+    return cd[..., :1] + cd[..., 1:] * z
+
+
+def _plain_load(st, pos):
+    case = st["case"]
+    r, ok = _rows(st, pos)
+    r = r.clamp(max=st["max_tok"] - 1)
+    s = torch.arange(case["slots"], device="cuda").view(-1, 1).expand_as(r)
+    for name, at in (("k_out", 0), ("v_out", BLK * ROW)):
+        codes, par = _parts(st, at)
+        x = _values(codes.permute(0, 2, 3, 1, 4)[s, r // BLK, r % BLK], par.permute(0, 2, 3, 1, 4)[s, r // BLK, r % BLK])
+        st[name].copy_(torch.where(ok.unsqueeze(-1), x.flatten(-2).to(st[name].dtype), st[name]))
+    return st["k_out"], st["v_out"]
+
+
+def _plain_attn(st):
+    case = st["case"]
+    S, T, H, M = case["slots"], case["T"], case["kv_heads"], st["max_tok"]
+    G = case["heads"] // H
+    kv = [_values(*_parts(st, at)).flatten(2, 3)[:, :, :M] for at in (0, BLK * ROW)]
+    i = torch.arange(T, device="cuda").view(1, T)
+    if st["pos"] is not None:
+        L = st["pos"].long().view(S, 1) + i + 1
+    elif st["lens"] is not None:
+        L = st["lens"].long().view(S, 1).expand(S, T)
+    else:
+        L = torch.full((S, T), M, device="cuda")
+    L = L.clamp(max=M)
+    if st["n"] is not None:
+        L = torch.where(i < st["n"].view(S, 1), L, 0)
+    in_cache = torch.arange(M, device="cuda").view(1, 1, M, 1) < L.amax(1).view(S, 1, 1, 1)
+    k, v = (torch.where(in_cache, x, 0.0) for x in kv)       # rows no query reaches may hold anything
+    mask = torch.arange(M, device="cuda").view(1, 1, M) < L.view(S, T, 1)              # [S][T][M]
+    q = st["q"].float().view(S, T, H, G, HD).permute(0, 2, 1, 3, 4).reshape(S, H, T * G, HD)
+    s = (q @ k.transpose(-1, -2)).mul_(1 / math.sqrt(HD)).view(S, H, T, G, M)
+    s.masked_fill_(~mask.view(S, 1, T, 1, M), float("-inf"))
+    mx = s.amax(-1, keepdim=True).clamp_(min=torch.finfo(torch.float32).min)
+    p = s.sub_(mx).exp_()
+    den = p.sum(-1, keepdim=True)
+    o = (p.view(S, H, T * G, M) @ v).view(S, H, T, G, HD) / torch.where(den > 0, den, 1.0)
+    o = o.permute(0, 2, 1, 3, 4).reshape(S, T, H * G * HD).to(st["out"].dtype)
+    if st["n"] is not None:
+        o = torch.where((i < st["n"].view(S, 1)).unsqueeze(-1), o, st["out"])
+    st["out"].copy_(o)
+    return st["out"]
+
+
+# ----------------------------------------------------------------------------- in 64 bits
+
+def _exact_row_values(block, at, rows, H):
+    """Slot's rows [len(rows)][H][64] in 64 bits, from its bytes [H][blocks][4608]."""
+    flat = block.reshape(H, -1)
+    base = (rows // BLK) * BLOCK_BYTES + at
+    byte = (base + (rows % BLK) * 32).view(-1, 1) + torch.arange(HD, device="cuda").view(1, -1) // 2
+    shift = 4 * (torch.arange(HD, device="cuda") % 2)
+    z = (flat[:, byte].to(torch.int32) >> shift) % 16 - 8
+    pair = (base + BLK * 32 + (rows % BLK) * 4).view(-1, 1) + torch.arange(4, device="cuda").view(1, -1)
+    cd = flat[:, pair].contiguous().view(torch.float16).double()
+    return (cd[..., 0:1] + cd[..., 1:2] * z.double()).transpose(0, 1)
+
+
+def _exact_quantised(x):
+    """The values that x [rows][64] reads back as."""
+    f = x.float()
+    lo = f.min(-1, keepdim=True).values
+    hi = f.max(-1, keepdim=True).values
+    c = (lo + (hi - lo) * torch.tensor(8 / 15, dtype=torch.float32, device=x.device)).half().double()
+    lo, hi, f = lo.double(), hi.double(), f.double()
+    need = torch.maximum((c - lo) / 8, (hi - c) / 7)
+    bits = need.view(torch.int64)
+    d = ((bits + (1 << 45) - 1) >> 45 << 45).view(torch.float64)     # eight significant bits, upward
+    d = torch.ceil(d * 2.0 ** 24) / 2.0 ** 24
+    t = f - c
+    z = torch.full_like(t, -8)
+    for j in range(-7, 8):
+        z += (t >= (j - 0.5) * d).double()
+    val = c + d * torch.where(d > 0, z, 0.0)
+    fits = ((f <= LIMIT) & (f >= -LIMIT)).all(-1, keepdim=True)
+    return torch.where(fits, val, float("nan"))
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    S, T, H, M = case["slots"], case["T"], case["kv_heads"], case["max_tok"]
+    first, n = _counts(case)
+    if case["op"] in ("store", "load"):
+        out = []
+        for name, at in (("k", 0), ("v", BLK * ROW)):
+            o = torch.zeros((S, T, H * HD), dtype=torch.float64, device="cuda")
+            for s in range(S):
+                m = min(n[s], M - first[s])
+                if case["op"] == "store":
+                    o[s, :m] = _exact_quantised(st[name][s, :m].reshape(-1, HD)).reshape(m, H * HD)
+                else:
+                    rows = torch.arange(m, device="cuda")
+                    o[s, :m] = _exact_row_values(st["data"][s], at, rows, H).reshape(m, H * HD)
+            out.append(o)
+        return tuple(out)
+    G, keys = case["heads"] // H, _keys(case)
+    out = torch.zeros((S, T, case["heads"], HD), dtype=torch.float64, device="cuda")
+    for s in range(S):
+        m = max(keys[s])
+        if m == 0:
+            continue
+        rows = torch.arange(m, device="cuda")
+        k, v = (_exact_row_values(st["data"][s], at, rows, H) for at in (0, BLK * ROW))
+        upto = torch.tensor(keys[s], device="cuda").view(-1, 1)
+        q = st["q"][s, :n[s]].double().view(n[s], case["heads"], HD)
+        for h in range(case["heads"]):
+            z = torch.einsum("td,md->tm", q[:, h], k[:, h // G]) * 0.125
+            z = torch.where(rows.view(1, -1) < upto, z, -math.inf)
+            out[s, :n[s], h] = torch.softmax(z, -1) @ v[:, h // G]
+    return out.reshape(S, T, -1)

@@ -6,6 +6,7 @@ A group is the 64 elements of one token and kv head: element i has the nibble n'
 nibble of byte i / 2 when i is even) and the value c + d n'.  With `own` false the operators
 run in their plain form on the same bytes; with `own` true through madi_b200.kv4.
 """
+import functools
 import math
 
 import torch
@@ -184,10 +185,18 @@ def prepare(case, seed):
 
 # ----------------------------------------------------------------------------- one pass
 
+@functools.lru_cache(None)
+def _kv4():
+    """The framework's module, the library bound to the device as a program does at its start."""
+    import madi_b200
+    madi_b200.init(torch.cuda.current_device())
+    return madi_b200.kv4
+
+
 def run(st):
     case = st["case"]
     if own:
-        from madi_b200 import kv4
+        kv4 = _kv4()
         cache = kv4.Cache(st["data"], st["max_tok"])
         if case["op"] == "store":
             kv4.store(cache, st["k"], st["v"], pos=st["pos"], n=st["n"])

@@ -349,6 +349,54 @@ int madi_flash_attn_enc(const uint16_t *q, const uint16_t *k, const uint16_t *v,
 int madi_self_attn(const float *q, const void *kc, const void *vc, int kv_dtype, const uint32_t *pos, int slots,
                    int heads, int kv_heads, int kv_dim, int max_tok, float *out, void *stream);
 
+/* ======================= K/V cache in 4 bits ================================= */
+/* No counterpart in the reference, whose caches are f32 (self) and f16 (cross).  One
+ * object holds K and V of every slot: the 64 elements of one (token, kv head) -- a group --
+ * as 64 four-bit codes and two f16 numbers (c, d), 36 bytes (f16: 128, f32: 256):
+ *   value = c + d * n',  n' in -8..7, every element within d / 2 of its value,
+ *   c = f16(lo + (hi - lo) * 8/15) (f32 steps) for lo, hi = min, max of the group,
+ *   d = the least number >= max((c - lo) / 8, (hi - c) / 7) with 8 significant bits that is
+ *       a multiple of 2^-24,  n' = floor((x - c) / d + 1/2) (0 where d = 0).
+ * A group with an element that is NaN, infinite or above 57344 in magnitude reads back as
+ * NaN.  Layout: [slot][kv head][ceil(max_tok / 64) blocks][4608 bytes], a block being
+ *   K codes [64][32] | K (c, d) [64][2] | V codes [64][32] | V (c, d) [64][2];
+ * element i of a group is nibble i % 2 (low first) of byte i / 2, holding n' + 8.
+ * data: madi_kv4_bytes(...) bytes of device memory owned by the caller, 16-byte aligned; it needs
+ * no initialisation (rows that were never stored are not attended).  head_dim 64. */
+typedef struct madi_kv4 {
+    uint8_t *data;
+    int32_t slots, kv_heads, max_tok;
+} madi_kv4;
+/* Bytes of such a cache; 0 for a bad shape (1 <= slots <= 65535, 1 <= kv_heads <= 1024,
+ * 1 <= max_tok <= 2^30). */
+size_t madi_kv4_bytes(int slots, int kv_heads, int max_tok);
+
+/* Quantise `rows` new K and V rows per slot into the cache: row i of slot s (i < n[s]) goes to
+ * cache row pos[s] + i of the same slot; rows at or past max_tok are dropped, all other rows
+ * of the cache stay as they are.  k, v: dtype MADI_F32 or MADI_F16, element (s, i, j) at
+ * s * slot_stride + i * row_stride + j, j < kv_heads * 64; 16-byte aligned rows.  pos, n: u32
+ * [slots] on the device (read there, so a graph can replay them); NULL: 0 and `rows`. */
+int madi_kv4_store(const madi_kv4 *c, const void *k, const void *v, int dtype, int rows, int64_t slot_stride,
+                   int64_t row_stride, const uint32_t *pos, const uint32_t *n, void *stream);
+
+/* The reverse: cache rows pos[s] + i into rows i < n[s] of k and v (f32 or f16, the value
+ * rounded once); rows past max_tok and rows i >= n[s] of k and v are left as they were. */
+int madi_kv4_load(const madi_kv4 *c, void *k, void *v, int dtype, int rows, int64_t slot_stride, int64_t row_stride,
+                  const uint32_t *pos, const uint32_t *n, void *stream);
+
+/* Attention of `rows` query rows per slot over the cache: row i of slot s, head h:
+ *   out = softmax(q . K^T / 8) V over the cache rows j < L of kv head h / (heads / kv_heads),
+ *   L = pos[s] + i + 1 (pos given: causal, the row at pos[s] + i the last one attended),
+ *       lens[s] (lens given), else max_tok; at most max_tok.  L = 0 gives a zero row.
+ * Query rows i >= n[s] are padding: their out rows are left as they were.  Rows past L are
+ * never used, whatever they hold.  q, out: dtype (both MADI_F32 or both MADI_F16), element
+ * (s, i, j) at s * slot + i * row, j < heads * 64, 16-byte aligned rows; out does not overlap
+ * q.  heads: a multiple of kv_heads, at most 1024.  pos, lens, n: u32 [slots] on the device or
+ * NULL; not both of pos and lens.  q must be finite. */
+int madi_kv4_attn(const madi_kv4 *c, const void *q, int dtype, int heads, int rows, int64_t q_slot, int64_t q_row,
+                  const uint32_t *pos, const uint32_t *lens, const uint32_t *n, void *out, int64_t o_slot,
+                  int64_t o_row, void *stream);
+
 /* The tail of a greedy token step for m slots in one launch, equal to madi_step_advance,
  * madi_logit_filter_rows (history tokens[s], step = the advanced pos[s]),
  * madi_suppress_rows (ids, may be NULL with n_suppress 0) and madi_argmax_conf in turn:

@@ -5,7 +5,7 @@ in include/madi_q8.h (libmadi_q8.so, CUDA kernels in madi_b200/csrc/), its
 Python binding (_lib), the host mirror of the reference's operator wrapper
 (backend) and a typed torch-facing API (q8).
 """
-from . import backend, q8  # noqa: F401
+from . import backend, kv4, q8  # noqa: F401
 from ._lib import MadiError, load  # noqa: F401
 
 

@@ -33,6 +33,12 @@ class madi_q8w(ctypes.Structure):
     _fields_ = [("qs", P), ("scales", P), ("n", ctypes.c_int32), ("k", ctypes.c_int32)]
 
 
+class madi_kv4(ctypes.Structure):
+    _fields_ = [("data", P), ("slots", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("max_tok", ctypes.c_int32)]
+
+
+I64 = ctypes.c_int64
+
 SIGNATURES = {
     "madi_init": ([I], I),
     "madi_cleanup": ([], None),
@@ -85,6 +91,10 @@ SIGNATURES = {
     "madi_merge_shard_argmax": ([P, P, I, I, P, P], I),
     "madi_cross_attn": ([P, P, P, I, I, I, I, I, I, P, P, P], I),
     "madi_self_attn": ([P, P, P, I, P, I, I, I, I, I, P, P], I),
+    "madi_kv4_bytes": ([I, I, I], SZ),
+    "madi_kv4_store": ([ctypes.POINTER(madi_kv4), P, P, I, I, I64, I64, P, P, P], I),
+    "madi_kv4_load": ([ctypes.POINTER(madi_kv4), P, P, I, I, I64, I64, P, P, P], I),
+    "madi_kv4_attn": ([ctypes.POINTER(madi_kv4), P, I, I, I, I64, I64, P, P, P, P, I64, I64, P], I),
     "madi_flash_attn_enc": ([P, P, P, I, P, I, I, I, I, P], I),
 }
 

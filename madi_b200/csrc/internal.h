@@ -164,6 +164,26 @@ cudaError_t launch_self_attn(float *out, const float *q, const void *kc, const v
 // ---- encoder self-attention on the tensor cores (flash_enc.cu); head_dim 64
 cudaError_t launch_flash_enc(const __half *q, const __half *k, const __half *v, int stride, __half *out,
                              int out_stride, int seq, int heads, int chunks, int *dev_err, cudaStream_t st);
+// ---- K/V cache in 4 bits (kv4.cu, kv4_attn.cu; format in kv4.cuh); head_dim 64
+struct Kv4Args {
+    uint8_t *data;                       // [slots][kv_heads][blocks of 64 tokens][4608]
+    int slots, kv_heads, max_tok;
+};
+// Strides in elements.  pos (first row per slot) and n (valid rows per slot) may be null.
+cudaError_t launch_kv4_store(const Kv4Args &a, const void *k, const void *v, bool f16, int rows, long long slot_stride,
+                             long long row_stride, const uint32_t *pos, const uint32_t *n, cudaStream_t st);
+cudaError_t launch_kv4_load(const Kv4Args &a, void *k, void *v, bool f16, int rows, long long slot_stride,
+                            long long row_stride, const uint32_t *pos, const uint32_t *n, cudaStream_t st);
+struct Kv4AttnArgs {
+    Kv4Args c;
+    const void *q;                       // f32 or f16 rows, as out
+    void *out;
+    int heads, rows;                     // query heads; query rows per slot
+    long long q_slot, q_row, o_slot, o_row;      // strides in elements
+    const uint32_t *pos, *lens, *n;      // at most one of pos and lens; each may be null
+    int *dev_err;
+};
+cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, bool f16, cudaStream_t st);
 // step_advance + logit_filter_indirect + suppress_list + argmax_conf for m slots in
 // one launch (V <= decode_tail_max_vocab()).
 int decode_tail_max_vocab();

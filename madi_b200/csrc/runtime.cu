@@ -1092,6 +1092,105 @@ int madi_self_attn(const float *q, const void *kc, const void *vc, int kv_dtype,
     return e == cudaSuccess ? MADI_OK : cuda_fail(e, "madi_self_attn");
 }
 
+namespace {
+constexpr int kKv4MaxRows = 1 << 20;
+constexpr int64_t kKv4MaxStride = 1ll << 40;
+size_t kv4_blocks(int max_tok) { return ((size_t)max_tok + 63) / 64; }
+bool kv4_shape_ok(int slots, int kv_heads, int max_tok) {
+    return slots >= 1 && slots <= 65535 && kv_heads >= 1 && kv_heads <= 1024 && max_tok >= 1 && max_tok <= (1 << 30);
+}
+// The cache and what the three entry points share.
+int kv4_check(const char *who, const madi_kv4 *c, int dtype, int rows) {
+    if (!S.ready) return fail(MADI_ENOINIT, "%s: not initialised", who);
+    if (!c || !c->data) return fail(MADI_EINVAL, "%s: null cache", who);
+    if (!kv4_shape_ok(c->slots, c->kv_heads, c->max_tok))
+        return fail(MADI_EINVAL, "%s: cache of %d slots, %d kv heads, %d tokens", who, c->slots, c->kv_heads, c->max_tok);
+    if (!aligned(c->data, 16)) return fail(MADI_EINVAL, "%s: the cache must be 16-byte aligned", who);
+    if (dtype != MADI_F32 && dtype != MADI_F16) return fail(MADI_EINVAL, "%s: dtype %d (MADI_F32 or MADI_F16)", who, dtype);
+    if (rows < 0 || rows > kKv4MaxRows) return fail(MADI_EINVAL, "%s: rows %d (0..%d)", who, rows, kKv4MaxRows);
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != S.device)
+        return fail(MADI_EINVAL, "%s: the current device is not device %d, which madi_init bound", who, S.device);
+    return MADI_OK;
+}
+// Row tensors: non-null, 16-byte aligned rows that do not overlap one another.
+int kv4_rows_check(const char *who, const char *what, const void *p, int dtype, int slots, int rows, int64_t slot,
+                   int64_t row, int64_t width) {
+    const int64_t unit = dtype == MADI_F32 ? 4 : 8;
+    if (!p) return fail(MADI_EINVAL, "%s: null %s", who, what);
+    if (!aligned(p, 16) || slot % unit || row % unit)
+        return fail(MADI_EINVAL, "%s: rows of %s must be 16-byte aligned", who, what);
+    if ((rows > 1 && (row < width || row > kKv4MaxStride)) ||
+        (slots > 1 && (slot < (rows > 1 ? (rows - 1) * row : 0) + width || slot > kKv4MaxStride)))
+        return fail(MADI_EINVAL, "%s: strides %lld / %lld of %s (rows of %lld)", who, (long long)slot, (long long)row, what,
+                    (long long)width);
+    return MADI_OK;
+}
+}  // namespace
+
+size_t madi_kv4_bytes(int slots, int kv_heads, int max_tok) {
+    return kv4_shape_ok(slots, kv_heads, max_tok) ? (size_t)slots * kv_heads * kv4_blocks(max_tok) * 4608 : 0;
+}
+
+int madi_kv4_store(const madi_kv4 *c, const void *k, const void *v, int dtype, int rows, int64_t slot_stride,
+                   int64_t row_stride, const uint32_t *pos, const uint32_t *n, void *stream) {
+    const char *who = "madi_kv4_store";
+    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
+    if (rows == 0) return MADI_OK;
+    for (const void *p : {k, v})
+        if (int rc = kv4_rows_check(who, p == k ? "k" : "v", p, dtype, c->slots, rows, slot_stride, row_stride,
+                                    (int64_t)c->kv_heads * 64))
+            return rc;
+    const Kv4Args a{c->data, c->slots, c->kv_heads, c->max_tok};
+    cudaError_t e = launch_kv4_store(a, k, v, dtype == MADI_F16, rows, slot_stride, row_stride, pos, n, pick_stream(stream));
+    return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
+}
+
+int madi_kv4_load(const madi_kv4 *c, void *k, void *v, int dtype, int rows, int64_t slot_stride, int64_t row_stride,
+                  const uint32_t *pos, const uint32_t *n, void *stream) {
+    const char *who = "madi_kv4_load";
+    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
+    if (rows == 0) return MADI_OK;
+    for (const void *p : {k, v})
+        if (int rc = kv4_rows_check(who, p == k ? "k" : "v", p, dtype, c->slots, rows, slot_stride, row_stride,
+                                    (int64_t)c->kv_heads * 64))
+            return rc;
+    if (k == v) return fail(MADI_EINVAL, "%s: k and v are the same buffer", who);
+    const Kv4Args a{c->data, c->slots, c->kv_heads, c->max_tok};
+    cudaError_t e = launch_kv4_load(a, k, v, dtype == MADI_F16, rows, slot_stride, row_stride, pos, n, pick_stream(stream));
+    return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
+}
+
+int madi_kv4_attn(const madi_kv4 *c, const void *q, int dtype, int heads, int rows, int64_t q_slot, int64_t q_row,
+                  const uint32_t *pos, const uint32_t *lens, const uint32_t *n, void *out, int64_t o_slot, int64_t o_row,
+                  void *stream) {
+    const char *who = "madi_kv4_attn";
+    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
+    if (heads <= 0 || heads > 1024 || heads % c->kv_heads)
+        return fail(MADI_EINVAL, "%s: %d heads over %d kv heads (a multiple, at most 1024)", who, heads, c->kv_heads);
+    if (pos && lens) return fail(MADI_EINVAL, "%s: both pos and lens", who);
+    if (rows == 0) return MADI_OK;
+    if (int rc = kv4_rows_check(who, "q", q, dtype, c->slots, rows, q_slot, q_row, (int64_t)heads * 64)) return rc;
+    if (int rc = kv4_rows_check(who, "out", out, dtype, c->slots, rows, o_slot, o_row, (int64_t)heads * 64)) return rc;
+    if (out == q) return fail(MADI_EINVAL, "%s: out is q", who);
+    Kv4AttnArgs a{};
+    a.c = Kv4Args{c->data, c->slots, c->kv_heads, c->max_tok};
+    a.q = q;
+    a.out = out;
+    a.heads = heads;
+    a.rows = rows;
+    a.q_slot = q_slot;
+    a.q_row = q_row;
+    a.o_slot = o_slot;
+    a.o_row = o_row;
+    a.pos = pos;
+    a.lens = lens;
+    a.n = n;
+    a.dev_err = S.dev_err;
+    cudaError_t e = launch_kv4_attn(a, dtype == MADI_F16, pick_stream(stream));
+    return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
+}
+
 int madi_step_advance(uint32_t *pos, int m, void *stream) {
     if (!S.ready) return fail(MADI_ENOINIT, "madi_step_advance: not initialised");
     if (!pos || m <= 0 || m > 32) return fail(MADI_EINVAL, "madi_step_advance: m=%d (1..32)", m);

@@ -371,18 +371,24 @@ typedef struct madi_kv4 {
  * 1 <= max_tok <= 2^30). */
 size_t madi_kv4_bytes(int slots, int kv_heads, int max_tok);
 
-/* Quantise `rows` new K and V rows per slot into the cache: row i of slot s (i < n[s]) goes to
- * cache row pos[s] + i of the same slot; rows at or past max_tok are dropped, all other rows
- * of the cache stay as they are.  k, v: dtype MADI_F32 or MADI_F16, element (s, i, j) at
- * s * slot_stride + i * row_stride + j, j < kv_heads * 64; 16-byte aligned rows.  pos, n: u32
- * [slots] on the device (read there, so a graph can replay them); NULL: 0 and `rows`. */
-int madi_kv4_store(const madi_kv4 *c, const void *k, const void *v, int dtype, int rows, int64_t slot_stride,
-                   int64_t row_stride, const uint32_t *pos, const uint32_t *n, void *stream);
+/* K and V rows beside the cache: element (s, i, j) of k and of v at s * slot_stride +
+ * i * row_stride + j, i < rows, j < kv_heads * 64; 16-byte aligned rows; dtype MADI_F32 or MADI_F16.
+ * Row i of slot s belongs to cache row pos[s] + i, for i < n[s].  pos, n: u32 [slots] on the device
+ * (read there, so a graph can replay them); NULL: 0 and `rows`. */
+typedef struct madi_kv4_rows {
+    void *k, *v;
+    const uint32_t *pos, *n;
+    int64_t slot_stride, row_stride;
+    int32_t dtype, rows;
+} madi_kv4_rows;
 
-/* The reverse: cache rows pos[s] + i into rows i < n[s] of k and v (f32 or f16, the value
- * rounded once); rows past max_tok and rows i >= n[s] of k and v are left as they were. */
-int madi_kv4_load(const madi_kv4 *c, void *k, void *v, int dtype, int rows, int64_t slot_stride, int64_t row_stride,
-                  const uint32_t *pos, const uint32_t *n, void *stream);
+/* Quantise the rows (read only) into the cache.  Rows at or past max_tok are dropped; all other
+ * rows of the cache stay as they are. */
+int madi_kv4_store(const madi_kv4 *c, const madi_kv4_rows *r, void *stream);
+
+/* The reverse: cache rows into r's rows, the value rounded once.  Rows past max_tok and rows
+ * i >= n[s] of k and v are left as they were. */
+int madi_kv4_load(const madi_kv4 *c, const madi_kv4_rows *r, void *stream);
 
 /* Attention of `rows` query rows per slot over the cache: row i of slot s, head h:
  *   out = softmax(q . K^T / 8) V over the cache rows j < L of kv head h / (heads / kv_heads),
@@ -392,10 +398,15 @@ int madi_kv4_load(const madi_kv4 *c, void *k, void *v, int dtype, int rows, int6
  * never used, whatever they hold.  q, out: dtype (both MADI_F32 or both MADI_F16), element
  * (s, i, j) at s * slot + i * row, j < heads * 64, 16-byte aligned rows; out does not overlap
  * q.  heads: a multiple of kv_heads, at most 1024.  pos, lens, n: u32 [slots] on the device or
- * NULL; not both of pos and lens.  q must be finite. */
-int madi_kv4_attn(const madi_kv4 *c, const void *q, int dtype, int heads, int rows, int64_t q_slot, int64_t q_row,
-                  const uint32_t *pos, const uint32_t *lens, const uint32_t *n, void *out, int64_t o_slot,
-                  int64_t o_row, void *stream);
+ * NULL; not both of pos and lens.  q must be finite.  Takes no scratch memory. */
+typedef struct madi_kv4_query {
+    const void *q;
+    void *out;
+    const uint32_t *pos, *lens, *n;
+    int64_t q_slot, q_row, o_slot, o_row;
+    int32_t dtype, heads, rows, reserved;
+} madi_kv4_query;
+int madi_kv4_attn(const madi_kv4 *c, const madi_kv4_query *a, void *stream);
 
 /* The tail of a greedy token step for m slots in one launch, equal to madi_step_advance,
  * madi_logit_filter_rows (history tokens[s], step = the advanced pos[s]),

@@ -33,12 +33,7 @@ class madi_q8w(ctypes.Structure):
     _fields_ = [("qs", P), ("scales", P), ("n", ctypes.c_int32), ("k", ctypes.c_int32)]
 
 
-class madi_kv4(ctypes.Structure):
-    _fields_ = [("data", P), ("slots", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("max_tok", ctypes.c_int32)]
-
-
-I64 = ctypes.c_int64
-
+# madi_kv4, madi_kv4_rows, madi_kv4_query: packed by the caller (kv4.py) and passed as bytes
 SIGNATURES = {
     "madi_init": ([I], I),
     "madi_cleanup": ([], None),
@@ -92,9 +87,9 @@ SIGNATURES = {
     "madi_cross_attn": ([P, P, P, I, I, I, I, I, I, P, P, P], I),
     "madi_self_attn": ([P, P, P, I, P, I, I, I, I, I, P, P], I),
     "madi_kv4_bytes": ([I, I, I], SZ),
-    "madi_kv4_store": ([ctypes.POINTER(madi_kv4), P, P, I, I, I64, I64, P, P, P], I),
-    "madi_kv4_load": ([ctypes.POINTER(madi_kv4), P, P, I, I, I64, I64, P, P, P], I),
-    "madi_kv4_attn": ([ctypes.POINTER(madi_kv4), P, I, I, I, I64, I64, P, P, P, P, I64, I64, P], I),
+    "madi_kv4_store": ([P, P, P], I),
+    "madi_kv4_load": ([P, P, P], I),
+    "madi_kv4_attn": ([P, P, P], I),
     "madi_flash_attn_enc": ([P, P, P, I, P, I, I, I, I, P], I),
 }
 

@@ -184,6 +184,8 @@ struct Kv4AttnArgs {
     int *dev_err;
 };
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, bool f16, cudaStream_t st);
+// Its form for many f16 query rows (kv4_flash.cu), chosen by launch_kv4_attn.
+cudaError_t launch_kv4_flash(const Kv4AttnArgs &a, cudaStream_t st);
 // step_advance + logit_filter_indirect + suppress_list + argmax_conf for m slots in
 // one launch (V <= decode_tail_max_vocab()).
 int decode_tail_max_vocab();

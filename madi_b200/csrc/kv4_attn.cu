@@ -513,6 +513,7 @@ cudaError_t launch_stream(const Kv4AttnArgs &a, cudaStream_t st) {
 
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, bool f16, cudaStream_t st) {
     const long long cols = (long long)a.rows * (a.heads / a.c.kv_heads);
+    if (f16 && cols >= 33) return launch_kv4_flash(a, st);
     if (f16)
         return cols <= 4 ? launch_stream<1, __half>(a, st)
                          : cols <= 8 ? launch_stream<2, __half>(a, st) : launch_stream<4, __half>(a, st);

@@ -1093,6 +1093,8 @@ int madi_self_attn(const float *q, const void *kc, const void *vc, int kv_dtype,
 }
 
 namespace {
+static_assert(sizeof(madi_kv4) == 24 && sizeof(madi_kv4_rows) == 56 && sizeof(madi_kv4_query) == 88,
+              "layouts packed by the Python binding");
 constexpr int kKv4MaxRows = 1 << 20;
 constexpr int64_t kKv4MaxStride = 1ll << 40;
 size_t kv4_blocks(int max_tok) { return ((size_t)max_tok + 63) / 64; }
@@ -1132,62 +1134,49 @@ size_t madi_kv4_bytes(int slots, int kv_heads, int max_tok) {
     return kv4_shape_ok(slots, kv_heads, max_tok) ? (size_t)slots * kv_heads * kv4_blocks(max_tok) * 4608 : 0;
 }
 
-int madi_kv4_store(const madi_kv4 *c, const void *k, const void *v, int dtype, int rows, int64_t slot_stride,
-                   int64_t row_stride, const uint32_t *pos, const uint32_t *n, void *stream) {
-    const char *who = "madi_kv4_store";
-    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
-    if (rows == 0) return MADI_OK;
-    for (const void *p : {k, v})
-        if (int rc = kv4_rows_check(who, p == k ? "k" : "v", p, dtype, c->slots, rows, slot_stride, row_stride,
-                                    (int64_t)c->kv_heads * 64))
+namespace {
+int kv4_copy(const char *who, const madi_kv4 *c, const madi_kv4_rows *r, bool store, void *stream) {
+    if (!r) return fail(MADI_EINVAL, "%s: null rows", who);
+    if (int rc = kv4_check(who, c, r->dtype, r->rows)) return rc;
+    if (r->rows == 0) return MADI_OK;
+    for (const void *p : {r->k, r->v})
+        if (int rc = kv4_rows_check(who, p == r->k ? "k" : "v", p, r->dtype, c->slots, r->rows, r->slot_stride,
+                                    r->row_stride, (int64_t)c->kv_heads * 64))
             return rc;
+    if (!store && r->k == r->v) return fail(MADI_EINVAL, "%s: k and v are the same buffer", who);
     const Kv4Args a{c->data, c->slots, c->kv_heads, c->max_tok};
-    cudaError_t e = launch_kv4_store(a, k, v, dtype == MADI_F16, rows, slot_stride, row_stride, pos, n, pick_stream(stream));
+    const bool f16 = r->dtype == MADI_F16;
+    cudaError_t e = store ? launch_kv4_store(a, r->k, r->v, f16, r->rows, r->slot_stride, r->row_stride, r->pos, r->n,
+                                             pick_stream(stream))
+                          : launch_kv4_load(a, r->k, r->v, f16, r->rows, r->slot_stride, r->row_stride, r->pos, r->n,
+                                            pick_stream(stream));
     return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
 }
+}  // namespace
 
-int madi_kv4_load(const madi_kv4 *c, void *k, void *v, int dtype, int rows, int64_t slot_stride, int64_t row_stride,
-                  const uint32_t *pos, const uint32_t *n, void *stream) {
-    const char *who = "madi_kv4_load";
-    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
-    if (rows == 0) return MADI_OK;
-    for (const void *p : {k, v})
-        if (int rc = kv4_rows_check(who, p == k ? "k" : "v", p, dtype, c->slots, rows, slot_stride, row_stride,
-                                    (int64_t)c->kv_heads * 64))
-            return rc;
-    if (k == v) return fail(MADI_EINVAL, "%s: k and v are the same buffer", who);
-    const Kv4Args a{c->data, c->slots, c->kv_heads, c->max_tok};
-    cudaError_t e = launch_kv4_load(a, k, v, dtype == MADI_F16, rows, slot_stride, row_stride, pos, n, pick_stream(stream));
-    return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
+int madi_kv4_store(const madi_kv4 *c, const madi_kv4_rows *r, void *stream) {
+    return kv4_copy("madi_kv4_store", c, r, true, stream);
 }
 
-int madi_kv4_attn(const madi_kv4 *c, const void *q, int dtype, int heads, int rows, int64_t q_slot, int64_t q_row,
-                  const uint32_t *pos, const uint32_t *lens, const uint32_t *n, void *out, int64_t o_slot, int64_t o_row,
-                  void *stream) {
+int madi_kv4_load(const madi_kv4 *c, const madi_kv4_rows *r, void *stream) {
+    return kv4_copy("madi_kv4_load", c, r, false, stream);
+}
+
+int madi_kv4_attn(const madi_kv4 *c, const madi_kv4_query *a, void *stream) {
     const char *who = "madi_kv4_attn";
-    if (int rc = kv4_check(who, c, dtype, rows)) return rc;
-    if (heads <= 0 || heads > 1024 || heads % c->kv_heads)
-        return fail(MADI_EINVAL, "%s: %d heads over %d kv heads (a multiple, at most 1024)", who, heads, c->kv_heads);
-    if (pos && lens) return fail(MADI_EINVAL, "%s: both pos and lens", who);
-    if (rows == 0) return MADI_OK;
-    if (int rc = kv4_rows_check(who, "q", q, dtype, c->slots, rows, q_slot, q_row, (int64_t)heads * 64)) return rc;
-    if (int rc = kv4_rows_check(who, "out", out, dtype, c->slots, rows, o_slot, o_row, (int64_t)heads * 64)) return rc;
-    if (out == q) return fail(MADI_EINVAL, "%s: out is q", who);
-    Kv4AttnArgs a{};
-    a.c = Kv4Args{c->data, c->slots, c->kv_heads, c->max_tok};
-    a.q = q;
-    a.out = out;
-    a.heads = heads;
-    a.rows = rows;
-    a.q_slot = q_slot;
-    a.q_row = q_row;
-    a.o_slot = o_slot;
-    a.o_row = o_row;
-    a.pos = pos;
-    a.lens = lens;
-    a.n = n;
-    a.dev_err = S.dev_err;
-    cudaError_t e = launch_kv4_attn(a, dtype == MADI_F16, pick_stream(stream));
+    if (!a) return fail(MADI_EINVAL, "%s: null query", who);
+    if (int rc = kv4_check(who, c, a->dtype, a->rows)) return rc;
+    if (a->heads <= 0 || a->heads > 1024 || a->heads % c->kv_heads)
+        return fail(MADI_EINVAL, "%s: %d heads over %d kv heads (a multiple, at most 1024)", who, a->heads, c->kv_heads);
+    if (a->pos && a->lens) return fail(MADI_EINVAL, "%s: both pos and lens", who);
+    if (a->rows == 0) return MADI_OK;
+    const int64_t w = (int64_t)a->heads * 64;
+    if (int rc = kv4_rows_check(who, "q", a->q, a->dtype, c->slots, a->rows, a->q_slot, a->q_row, w)) return rc;
+    if (int rc = kv4_rows_check(who, "out", a->out, a->dtype, c->slots, a->rows, a->o_slot, a->o_row, w)) return rc;
+    if (a->out == a->q) return fail(MADI_EINVAL, "%s: out is q", who);
+    const Kv4AttnArgs k{{c->data, c->slots, c->kv_heads, c->max_tok}, a->q, a->out, a->heads, a->rows, a->q_slot, a->q_row,
+                        a->o_slot, a->o_row, a->pos, a->lens, a->n, S.dev_err};
+    cudaError_t e = launch_kv4_attn(k, a->dtype == MADI_F16, pick_stream(stream));
     return e == cudaSuccess ? MADI_OK : cuda_fail(e, who);
 }
 

@@ -128,7 +128,7 @@ def _attn_case(madi, slots, rows, heads, kv_heads, max_tok, dt, pos=None, lens=N
     written = [max([int(v) for v in L[s, :nn[s]]], default=0) for s in range(slots)]
     data = R.random_cache(g, slots, kv_heads, max_tok, written, spread)
     q = (g.standard_normal((slots, rows, heads * 64)) * qscale).astype(dt)
-    p16 = False
+    p16 = dt == F16                # the many-row form rounds its weights to f16
     want, tol = R.attend(q, data, max_tok, heads, L, n, f16=dt == F16, p16=p16)
     Q = _t(q)
     out = torch.full(Q.shape, 5.0, dtype=Q.dtype, device="cuda")

@@ -1,7 +1,5 @@
 """CPU: what the 4-bit K/V cache's entry points refuse before any launch, and the format's own
 promises (64-bit definition in kv4_ref)."""
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -47,7 +45,7 @@ def _raises(match, fn, *a, **k):
 def test_store_and_load_refusals():
     c, x = _cache(), torch.zeros((2, 5, 192))
     i = torch.zeros(2, dtype=torch.int32)
-    _raises("CUDA device", kv4.store, c, x, x)                             # a cache in host memory
+    _raises("host memory", kv4.store, c, x, x)                             # a cache in host memory
     _raises("k must be", kv4.store, c, x[:1], x[:1])
     _raises("k must be", kv4.store, c, x[..., :128], x[..., :128])
     _raises("k must be", kv4.store, c, x.double(), x.double())
@@ -60,7 +58,7 @@ def test_store_and_load_refusals():
         for bad in (i.long(), i[:1], torch.zeros((2, 1), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)[::2]):
             _raises(name, kv4.store, c, x, x, **{name: bad})
             _raises(name, kv4.load, c, 5, k_out=x, v_out=x.clone(), **{name: bad})
-    _raises("CUDA device", kv4.load, c, 5, k_out=x, v_out=x.clone())
+    _raises("host memory", kv4.load, c, 5, k_out=x, v_out=x.clone())
     _raises("go together", kv4.load, c, 5, k_out=x)
     _raises("holds 5 rows", kv4.load, c, 4, k_out=x, v_out=x.clone())
     _raises("v_out must match", kv4.load, c, 5, k_out=x, v_out=x.half())
@@ -71,7 +69,7 @@ def test_store_and_load_refusals():
 def test_attn_refusals():
     c, q = _cache(), torch.zeros((2, 6 * 64))
     i = torch.zeros(2, dtype=torch.int32)
-    _raises("CUDA device", kv4.attn, q, c, 6)
+    _raises("host memory", kv4.attn, q, c, 6)
     _raises("q must be", kv4.attn, q, c, 3)
     _raises("q must be", kv4.attn, q.double(), c, 6)
     _raises("q must be", kv4.attn, q[:1], c, 6)
@@ -89,10 +87,11 @@ def test_calls_before_init_fail_cleanly():
     if torch.cuda.is_available():
         pytest.skip("another test may have initialised the library")
     L = _lib.load()
-    h = _lib.madi_kv4(4096, 1, 1, 64)
-    assert L.madi_kv4_store(ctypes.byref(h), 4096, 4096, 0, 1, 64, 64, None, None, None) == _lib.MADI_ENOINIT
-    assert L.madi_kv4_load(ctypes.byref(h), 4096, 8192, 0, 1, 64, 64, None, None, None) == _lib.MADI_ENOINIT
-    assert L.madi_kv4_attn(ctypes.byref(h), 4096, 0, 1, 1, 64, 64, None, None, None, 8192, 64, 64, None) == _lib.MADI_ENOINIT
+    h, x = kv4._CACHE(4096, 1, 1, 64), kv4._ROWS(4096, 8192, 0, 0, 64, 64, 0, 1)
+    q = kv4._QUERY(4096, 8192, 0, 0, 0, 64, 64, 64, 64, 0, 1, 1, 0)
+    for f, a in ((L.madi_kv4_store, x), (L.madi_kv4_load, x), (L.madi_kv4_attn, q)):
+        assert f(h, a, None) == _lib.MADI_ENOINIT
+        assert f(h, None, None) == _lib.MADI_EINVAL
 
 
 def test_format_promises():

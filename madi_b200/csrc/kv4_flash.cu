@@ -1,23 +1,23 @@
 // kv4_flash.cu -- attention of many query rows over the 4-bit K/V cache (kv4.cuh) on the
 // 5th-generation tensor cores: f16 queries and outputs, head_dim 64.
 //
-// Same mathematics as the streaming form (kv4_attn.cu), as matrix products of 128 x 128 tiles:
+// Same mathematics as the streaming form (kv4_attn.cu), as matrix products of 128 x 96 tiles:
 //     S = Q K^T,  K = c + d n':   Q (d n')^T + sum(Q) c^T
 //     O = P V,    V = c + d n':   P (d n')   + sum_j P_j c_j
 // d has 8 significant bits and |n'| <= 8, so d n' is exact in f16 and only P is rounded (2^-11 at
 // most, as the output itself is): the keys' c enters S as a fifth K = 16 step with sum(Q) as two
-// f16 parts, the values' c as one f32 FMA per score beside the softmax.  Rounding c + d n' to f16
-// instead would add two more errors of the output's own size.
+// f16 parts, the values' c as one more column of V, beside a column of ones that gives the sum of
+// the weights.  Rounding c + d n' to f16 instead would add two more errors of the output's own size.
 //
 // One CTA per (256 query columns of one kv head, slot, share of the keys); a column is one
-// (query row, query head of the kv head).  13 warps:
-//   warps 0-3   one key per thread: read its packed K and V (64 bytes and two (c, d)), write the two
-//               f16 rows and the c's into a 3-stage ring, in the SWIZZLE_128B layout; the next
-//               tile's bytes are in flight meanwhile;
+// (query row, query head of the kv head).  Warps:
+//   warps 0-2   read the packed K and V rows (32 bytes and (c, d) each), write the f16 rows and the
+//               c's into a 3-stage ring, in the SWIZZLE_128B layout; the next tile's bytes are in
+//               flight meanwhile;
+//   warp 3      issues the products (S: 5 steps, both operands in shared memory; O: P in TMEM as
+//               the first operand, V N-contiguous) and owns TMEM;
 //   warps 4-11  the softmax of the two 128-column tiles (thread = column = TMEM lane), as in
-//               flash_enc.cu: S in TMEM, P written back as f16, O rescaled when a maximum grew;
-//   warp 12     issues the products (S: 5 steps, both operands in shared memory; O: P in TMEM as
-//               the first operand, V N-contiguous) and owns TMEM.
+//               flash_enc.cu: S in TMEM, P written back as f16, O rescaled when a maximum grew.
 // Within every 8 dims the shared-memory order is 0 4 1 5 2 6 3 7 -- what one mask of a code word
 // gives as a pair of f16 -- for Q and K alike, and for V's columns, which are put back in order
 // when O is written.  Each query row is scaled by a power of two so that its largest element lies
@@ -31,8 +31,8 @@
 #include <math_constants.h>
 #include <stdint.h>
 
-#include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "internal.h"
 #include "kv4.cuh"
@@ -43,25 +43,26 @@ namespace madi {
 namespace {
 
 constexpr int kQT = 128;                       // query columns per tile
-constexpr int kKT = 128;                       // keys per tile
+constexpr int kKT = 96;                        // keys per tile: S, P and O of two tiles fit TMEM, a row of S registers
 constexpr int kNS = 3;                         // ring stages
-constexpr int kTile = 128 * 64 * 2;            // bytes of one [128][64] f16 tile
-constexpr int kDeqThr = 128;                   // warps 0..3
+constexpr int kTile = 128 * 64 * 2;            // bytes of one [128][64] f16 tile (Q)
+constexpr int kKTile = kKT * 64 * 2;           // bytes of one [96][64] f16 tile (K, V)
+constexpr int kDeqThr = 96;                    // warps 0..2
+constexpr int kMmaWarp = 3;
 constexpr int kSmWarp0 = 4;                    // warps 4..7: tile 0; 8..11: tile 1
-constexpr int kMmaWarp = 12;
-constexpr int kThr = 32 * 13;
+constexpr int kThr = 32 * 12;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kTileCols = 256, kPCol = 128, kOCol = 192;
+constexpr uint32_t kTileCols = 256, kPCol = 96, kOCol = 144, kSumCol = kOCol + kKv4Hd;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kIdescS = idesc_f16_f32(kQT, kKT);
-constexpr uint32_t kIdescPV = idesc_f16_f32(kQT, kKv4Hd) | (1u << 16);     // V: N-contiguous
+constexpr uint32_t kIdescPV = idesc_f16_f32(kQT, kKv4Hd + 16) | (1u << 16);      // V: N-contiguous
 constexpr int kMaxNs = 8;
+constexpr float kSlack = 8.f;                  // base-2 head room of the softmax reference
 constexpr int kPartW = kKv4Hd + 2;             // a row's partial: O, m, l
 
 struct __align__(16) FlashShared {
-    float cv[kNS][kKT];      // the values' c
     uint64_t q_full;         // 256: both Q tiles and their sums written
-    uint64_t kv_full[kNS];   // 128: a stage's keys and values written
+    uint64_t kv_full[kNS];   // 96: a stage's keys and values written
     uint64_t kv_empty[kNS];  // its products complete
     uint64_t s_full[2], s_free[2], p_ready[2], o_done[2];
     uint64_t drain;
@@ -70,8 +71,9 @@ struct __align__(16) FlashShared {
 };
 
 // Q tiles 0 and 1 | sums of Q (tile x in 16-byte chunks 2x, 2x + 1 of each row) | stages of
-// K, c of K (chunks 0, 1 of each row), V.
-constexpr size_t kQBytes = 3 * (size_t)kTile, kStage = 3 * (size_t)kTile;
+// K | V | a key's extra columns, in one row: chunks 0, 1 the columns 64.. of V (the value's c, then
+// 1: their products with P are sum p c and sum p), chunks 2, 3 the fifth step of K (c twice).
+constexpr size_t kQBytes = 3 * (size_t)kTile, kStage = 3 * (size_t)kKTile;
 constexpr size_t kSmem = 1024 + kQBytes + kNS * kStage + sizeof(FlashShared);
 static_assert(kSmem <= 227 * 1024, "shared memory");
 static_assert(kNS * kStage >= 2 * kQT * kPartW * sizeof(float), "the partials take the ring's place");
@@ -88,6 +90,13 @@ MADI_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+// Two consecutive 32-bit columns.
+MADI_DEV void tmem_ld2(uint32_t taddr, uint32_t &r0, uint32_t &r1) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(taddr));
+}
+MADI_DEV void tmem_st2(uint32_t taddr, uint32_t r0, uint32_t r1) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(r0), "r"(r1) : "memory");
+}
 MADI_DEV float max3f(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -95,7 +104,7 @@ MADI_DEV float max3f(float a, float b, float c) {
 }
 MADI_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 16-byte chunk c of row r of a [128][64] f16 tile in the SWIZZLE_128B layout.
+// 16-byte chunk c of row r of a [..][64] f16 tile in the SWIZZLE_128B layout.
 MADI_DEV uint4 *chunk(uint8_t *tile, int r, int c) {
     return reinterpret_cast<uint4 *>(tile + r * 128 + ((c ^ (r & 7)) << 4));
 }
@@ -116,9 +125,10 @@ MADI_DEV uint4 dequant_word(uint32_t w, __half2 d) {
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-struct KeyBytes {
-    uint4 k0, k1, v0, v1;
-    uint32_t kcd, vcd;
+MADI_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<__half2 *>(&w); }
+struct RowBytes {
+    uint4 lo, hi;       // code words
+    uint32_t cd;
 };
 
 __global__ void __launch_bounds__(kThr, 1)
@@ -174,71 +184,70 @@ __global__ void __launch_bounds__(kThr, 1)
     const uint32_t tmem = sh->tmem_base;
     volatile int *abort_flag = &sh->abort;
 
-    // softmax state, kept to the end of the kernel
-    float m = -CUDART_INF_F, l = 0.f, oc = 0.f;
-    const int x = warp >= kSmWarp0 + 4 ? 1 : 0;              // column tile of a softmax warp
-    const int row = (warp & 3) * 32 + lane;                  // column within the tile
-    const uint32_t tb = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kTileCols;
-    const int col = col0 + x * kQT + row;
-    bool alive = true;
-
-    if (warp < 4) {
-        // ------------------------------------------------ codes -> f16 tiles, one key per thread
+    if (warp < kMmaWarp) {
+        // ------------------------------------------------ codes -> f16 tiles
+        // One key per thread: its K and V rows, fetched a tile ahead as soon as the ones before are
+        // written, so that one set of registers serves.
         const int r = threadIdx.x;
         const uint8_t *src = a.c.data + s * slot_bytes + kvh * head_bytes;
-        auto fetch = [&](int j, KeyBytes &b) {
+        RowBytes kb, vb;
+        auto fetch = [&](int j, int half, RowBytes &b) {
             const int key = (j0 + j) * kKT + r;
-            b.kcd = b.vcd = 0;
-            if (key < kmax) {
-                const uint8_t *blk = src + (long long)(key / kKv4Blk) * kKv4Block;
+            b.lo = b.hi = make_uint4(0, 0, 0, 0);
+            b.cd = 0;                                        // d = 0: a zero row
+            if (j < nmax && key < kmax) {
+                const uint8_t *blk = src + (long long)(key / kKv4Blk) * kKv4Block + half;
                 const int off = key % kKv4Blk;
-                const uint4 *kp = reinterpret_cast<const uint4 *>(blk + off * 32);
-                const uint4 *vp = reinterpret_cast<const uint4 *>(blk + kKv4Half + off * 32);
-                b.k0 = kp[0];
-                b.k1 = kp[1];
-                b.v0 = vp[0];
-                b.v1 = vp[1];
-                b.kcd = *reinterpret_cast<const uint32_t *>(blk + kKv4Codes + off * 4);
-                b.vcd = *reinterpret_cast<const uint32_t *>(blk + kKv4Half + kKv4Codes + off * 4);
-            } else {
-                b.k0 = b.k1 = b.v0 = b.v1 = make_uint4(0, 0, 0, 0);      // d = 0: a zero row
+                b.lo = reinterpret_cast<const uint4 *>(blk + off * 32)[0];
+                b.hi = reinterpret_cast<const uint4 *>(blk + off * 32)[1];
+                b.cd = *reinterpret_cast<const uint32_t *>(blk + kKv4Codes + off * 4);
             }
         };
-        for (int i = 0; i < kNS; ++i) *chunk(ring + i * kStage + kTile, r, 1) = make_uint4(0, 0, 0, 0);
-        KeyBytes b;
-        if (nmax > 0) fetch(0, b);
+        auto write = [&](uint8_t *rows, const RowBytes &b, __half2 d) {
+            const uint32_t w[8] = {b.lo.x, b.lo.y, b.lo.z, b.lo.w, b.hi.x, b.hi.y, b.hi.z, b.hi.w};
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *chunk(rows, r, c) = dequant_word(w[c], d);
+        };
+        for (int i = 0; i < kNS; ++i) {
+            *chunk(ring + i * kStage + 2 * kKTile, r, 1) = make_uint4(0, 0, 0, 0);
+            *chunk(ring + i * kStage + 2 * kKTile, r, 3) = make_uint4(0, 0, 0, 0);
+        }
+        fetch(0, 0, kb);
+        fetch(0, kKv4Half, vb);
         for (int j = 0; j < nmax; ++j) {
             const int st = j % kNS;
             if (!warp_wait_all(&sh->kv_empty[st], ((uint32_t)(j / kNS) & 1u) ^ 1u, abort_flag, a.dev_err)) break;
-            const KeyBytes cur = b;
-            if (j + 1 < nmax) fetch(j + 1, b);
-            uint8_t *kt = ring + st * kStage, *kx = kt + kTile, *vt = kx + kTile;
-            __half2 kcd = *reinterpret_cast<const __half2 *>(&cur.kcd), vcd = *reinterpret_cast<const __half2 *>(&cur.vcd);
+            uint8_t *kt = ring + st * kStage, *xt = kt + 2 * kKTile;
+            __half2 kcd = as_h2(kb.cd), vcd = as_h2(vb.cd);
             // A value row that reads back as NaN must reach the columns that attend it and no
             // other: P = 0 times NaN would reach all.  It makes its key's score NaN instead.
-            const float vc = __low2float(vcd), vd = __high2float(vcd);
-            if (!(fabsf(vc) <= 65504.f && fabsf(vd) <= 65504.f)) {
+            if (!(fabsf(__low2float(vcd)) <= 65504.f && fabsf(__high2float(vcd)) <= 65504.f)) {
                 vcd = __float2half2_rn(0.f);
                 kcd = __halves2half2(__float2half_rn(CUDART_NAN_F), __high2half(kcd));
             }
-            const __half2 kd = __high2half2(kcd), vd2 = __high2half2(vcd);
-            const uint32_t kw[8] = {cur.k0.x, cur.k0.y, cur.k0.z, cur.k0.w, cur.k1.x, cur.k1.y, cur.k1.z, cur.k1.w};
-            const uint32_t vw[8] = {cur.v0.x, cur.v0.y, cur.v0.z, cur.v0.w, cur.v1.x, cur.v1.y, cur.v1.z, cur.v1.w};
-#pragma unroll
-            for (int c = 0; c < 8; ++c) *chunk(kt, r, c) = dequant_word(kw[c], kd);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) *chunk(vt, r, c) = dequant_word(vw[c], vd2);
-            *chunk(kx, r, 0) = make_uint4(h2_as_u32(__low2half2(kcd)), 0, 0, 0);
-            sh->cv[st][r] = __low2float(vcd);
+            write(kt, kb, __high2half2(kcd));
+            fetch(j + 1, 0, kb);
+            write(kt + kKTile, vb, __high2half2(vcd));
+            fetch(j + 1, kKv4Half, vb);
+            *chunk(xt, r, 0) = make_uint4(h2_as_u32(__halves2half2(__low2half(vcd), __float2half_rn(1.f))), 0, 0, 0);
+            *chunk(xt, r, 2) = make_uint4(h2_as_u32(__low2half2(kcd)), 0, 0, 0);
             fence_proxy_async_smem();
             mbar_arrive(&sh->kv_full[st]);
+        }
+        if (ns > 1) {                                        // the softmax warps' join
+            named_bar_sync(0, kThr);
+            cluster_sync_all();
+            cluster_sync_all();
         }
     } else if (warp == kMmaWarp) {
         // ------------------------------------------------ products
         if (lane == 0) {
             const uint64_t qd = smem_desc_sw128(smem_u32(qs)), qxd = smem_desc_sw128(smem_u32(qx));
             const uint64_t rd = smem_desc_sw128(smem_u32(ring));
-            constexpr uint64_t kTileU = kTile >> 4, kStageU = kStage >> 4;
+            constexpr uint64_t kTileU = kTile >> 4, kKTileU = kKTile >> 4, kStageU = kStage >> 4;
+            // V N-contiguous: its columns 64.. lie one [96][64] tile further on (the descriptor's leading
+            // offset, bits 16..29, which K-major operands do not use)
+            const uint64_t vd = (rd & ~((uint64_t)0x3FFF << 16)) + kKTileU + (kKTileU << 16);
             int seen = -1;                                   // last key tile known to be in the ring
             bool ok = mbar_wait(&sh->q_full, 0, abort_flag, a.dev_err);
             auto issue_s = [&](int y, int j) -> bool {
@@ -252,7 +261,7 @@ __global__ void __launch_bounds__(kThr, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     mma_ss(tmem + y * kTileCols, qd + y * kTileU + 2 * k, kd + 2 * k, kIdescS, k != 0);
-                mma_ss(tmem + y * kTileCols, qxd + 2 * y, kd + kTileU, kIdescS, 1);
+                mma_ss(tmem + y * kTileCols, qxd + 2 * y, kd + 2 * kKTileU + 2, kIdescS, 1);
                 umma_commit(&sh->s_full[y]);
                 return true;
             };
@@ -275,7 +284,7 @@ __global__ void __launch_bounds__(kThr, 1)
                     const uint32_t t0 = tmem + y * kTileCols;
 #pragma unroll
                     for (int k = 0; k < kKT / 16; ++k)
-                        umma_f16_ts(t0 + kOCol, t0 + kPCol + 8 * k, rd + st * kStageU + 2 * kTileU + 128 * k, kIdescPV,
+                        umma_f16_ts(t0 + kOCol, t0 + kPCol + 8 * k, vd + st * kStageU + 128 * k, kIdescPV,
                                     (j | k) != 0);
                     umma_commit(&sh->o_done[y]);
                 }
@@ -285,8 +294,19 @@ __global__ void __launch_bounds__(kThr, 1)
             wait_drain(&sh->drain, 0);
         }
         __syncwarp();
+        if (ns > 1) {                                        // the softmax warps' join
+            named_bar_sync(0, kThr);
+            cluster_sync_all();
+            cluster_sync_all();
+        }
     } else {
         // ------------------------------------------------ softmax, one query column per thread
+        float m = -CUDART_INF_F;
+        const int x = warp >= kSmWarp0 + 4 ? 1 : 0;          // column tile of this warp
+        const int row = (warp & 3) * 32 + lane;              // column within the tile
+        const uint32_t tb = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kTileCols;
+        const int col = col0 + x * kQT + row;
+        bool alive = true;
         const int q = col / group;
         const bool real = col < total;
         const int klim = real ? kv4_keys(a.pos, a.lens, s, q, a.c.max_tok) : 0x7fffffff;
@@ -335,86 +355,59 @@ __global__ void __launch_bounds__(kThr, 1)
         }
         const int n = nt[x];
         for (int j = 0; j < n; ++j) {
-            const int st = j % kNS;
-            alive = warp_wait_all(&sh->s_full[x], (uint32_t)j & 1u, abort_flag, a.dev_err) &&
-                    warp_wait_all(&sh->kv_full[st], (uint32_t)(j / kNS) & 1u, abort_flag, a.dev_err);
+            alive = warp_wait_all(&sh->s_full[x], (uint32_t)j & 1u, abort_flag, a.dev_err);
             if (!alive) break;
             tc_fence_after();
             const int kcur = klim - min((j0 + j) * kKT, klim);           // keys of this tile the column attends
             const bool full = __all_sync(0xffffffffu, kcur >= kKT);
-            float mx[8];
+            float mn = m, alpha = 1.f;
+            // One row of S through the softmax.  Only the last tiles of a column mask keys: their own
+            // copy of the code, so that the others carry no selects.
+            auto tile_softmax = [&](auto whole) -> bool {
+                uint32_t sv[kKT / 32][32];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx[k] = -CUDART_INF_F;
-            uint32_t sv[2][32];
-            tmem_ld32(tb, sv[0]);
-            tmem_wait_ld();
+                for (int c = 0; c < kKT / 32; ++c) tmem_ld32(tb + 32 * c, sv[c]);
+                tmem_wait_ld();
+                tc_fence_before();                           // S is in registers: the next S may take its place
+                mbar_arrive(&sh->s_free[x]);
+                auto score = [&](int c, int i) {
+                    const float v = __uint_as_float(sv[c][i]);
+                    return whole.value || 32 * c + i < kcur ? v : -CUDART_INF_F;
+                };
+                float mx[8];
 #pragma unroll
-            for (int c = 0; c < kKT / 32; ++c) {
-                if (c + 1 < kKT / 32) tmem_ld32(tb + 32 * (c + 1), sv[(c + 1) & 1]);
-                const uint32_t (&cv)[32] = sv[c & 1];
-                if (full) {
+                for (int k = 0; k < 8; ++k) mx[k] = -CUDART_INF_F;
+#pragma unroll
+                for (int c = 0; c < kKT / 32; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
-                        mx[(i >> 1) & 7] = max3f(mx[(i >> 1) & 7], __uint_as_float(cv[i]), __uint_as_float(cv[i + 1]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * c + i < kcur) mx[i & 7] = fmaxf(mx[i & 7], __uint_as_float(cv[i]));
+                        mx[(i >> 1) & 7] = max3f(mx[(i >> 1) & 7], score(c, i), score(c, i + 1));
+                const float mxr = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                // The reference moves only when a maximum passes it by more than 2^kSlack: weights up
+                // to 2^kSlack are as good in f16 and f32, and O is rescaled in few tiles instead of most.
+                const float mt = mxr * scale;
+                mn = mt > m + kSlack ? mt : m;
+                const float ml = mn == -CUDART_INF_F ? 0.f : mn;          // no key yet
+                alpha = mn == m ? 1.f : ex2_approx(m - ml);               // exactly 1 when it did not move
+                if (j > 0) {
+                    if (!warp_wait_all(&sh->o_done[x], (uint32_t)(j - 1) & 1u, abort_flag, a.dev_err)) return false;
+                    tc_fence_after();
                 }
-                if (c + 1 < kKT / 32) tmem_wait_ld();
-            }
-            const float mxr =
-                fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-            const float mn = fmaxf(m, mxr * scale);
-            const float ml = mn == -CUDART_INF_F ? 0.f : mn;              // no key yet
-            const float alpha = mn == m ? 1.f : ex2_approx(m - ml);       // exactly 1 when it did not move
-            if (j > 0) {
-                alive = warp_wait_all(&sh->o_done[x], (uint32_t)(j - 1) & 1u, abort_flag, a.dev_err);
-                if (!alive) break;
-                tc_fence_after();
-            }
-            float bq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, bc[4] = {0.f, 0.f, 0.f, 0.f};
-            tmem_ld32(tb, sv[0]);
-            tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < kKT / 32; ++c) {
-                if (c + 1 < kKT / 32) tmem_ld32(tb + 32 * (c + 1), sv[(c + 1) & 1]);
-                const uint32_t (&cv)[32] = sv[c & 1];
-                uint32_t pp[16];
+                for (int c = 0; c < kKT / 32; ++c) {
+                    uint32_t pp[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 cc = *reinterpret_cast<const float4 *>(&sh->cv[st][32 * c + i]);
-                    float e[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2) {
+                    for (int i = 0; i < 32; i += 2) {
                         float a0, a1;
-                        fma2(a0, a1, __uint_as_float(cv[i + k]), __uint_as_float(cv[i + k + 1]), scale, scale, -ml, -ml);
-                        e[k] = ex2_approx(a0);
-                        e[k + 1] = ex2_approx(a1);
+                        fma2(a0, a1, score(c, i), score(c, i + 1), scale, scale, -ml, -ml);
+                        pp[i >> 1] = h2_as_u32(__floats2half2_rn(ex2_approx(a0), ex2_approx(a1)));
                     }
-                    if (!full) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) e[k] = 32 * c + i + k < kcur ? e[k] : 0.f;
-                    }
-                    const int g = (i >> 1) & 2;
-                    add2(bq[2 * g], bq[2 * g + 1], bq[2 * g], bq[2 * g + 1], e[0], e[1]);
-                    add2(bq[2 * g + 2], bq[2 * g + 3], bq[2 * g + 2], bq[2 * g + 3], e[2], e[3]);
-                    fma2(bc[0], bc[1], e[0], e[1], cc.x, cc.y, bc[0], bc[1]);
-                    fma2(bc[2], bc[3], e[2], e[3], cc.z, cc.w, bc[2], bc[3]);
-                    pp[i >> 1] = h2_as_u32(__floats2half2_rn(e[0], e[1]));
-                    pp[(i >> 1) + 1] = h2_as_u32(__floats2half2_rn(e[2], e[3]));
+                    tmem_st16(tb + kPCol + 16 * c, pp);
                 }
-                tmem_st16(tb + kPCol + 16 * c, pp);
-                if (c + 1 < kKT / 32) {
-                    tmem_wait_ld();
-                    if (c + 2 == kKT / 32) {
-                        tc_fence_before();                   // the last of S is in registers
-                        mbar_arrive(&sh->s_free[x]);
-                    }
-                }
-            }
-            l = l * alpha + (((bq[0] + bq[1]) + (bq[2] + bq[3])) + ((bq[4] + bq[5]) + (bq[6] + bq[7])));
-            oc = oc * alpha + ((bc[0] + bc[1]) + (bc[2] + bc[3]));
+                return true;
+            };
+            alive = full ? tile_softmax(std::true_type{}) : tile_softmax(std::false_type{});
+            if (!alive) break;
             const bool grew = mn != m;
             m = mn;
             if (j > 0 && __any_sync(0xffffffffu, grew)) {
@@ -432,13 +425,27 @@ __global__ void __launch_bounds__(kThr, 1)
                     }
                     tmem_st32(tb + kOCol + 32 * c, ov);
                 }
+                uint32_t c0, c1;
+                tmem_ld2(tb + kSumCol, c0, c1);
+                tmem_wait_ld();
+                tmem_st2(tb + kSumCol, __float_as_uint(__uint_as_float(c0) * alpha), __float_as_uint(__uint_as_float(c1) * alpha));
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&sh->p_ready[x]);
         }
         if (alive && n > 0) alive = warp_wait_all(&sh->o_done[x], (uint32_t)(n - 1) & 1u, abort_flag, a.dev_err);
-        if (alive) tc_fence_after();
+        float l = 0.f, oc = 0.f;                             // sums of p and of p c
+        if (alive) {
+            tc_fence_after();
+            if (n > 0) {
+                uint32_t c0, c1;
+                tmem_ld2(tb + kSumCol, c0, c1);
+                tmem_wait_ld();
+                oc = __uint_as_float(c0);
+                l = __uint_as_float(c1);
+            }
+        }
         if (ns == 1 && alive) {
             // O columns 8 g + 2 r, 8 g + 2 r + 1 are dims 8 g + r, 8 g + r + 4
             const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -472,16 +479,13 @@ __global__ void __launch_bounds__(kThr, 1)
                 }
             }
         }
-    }
-
-    if (ns > 1) {
-        // The cluster's partials: this CTA's rows into the ring's place (its products are
-        // done), then every CTA joins its share of the rows from all of them.
-        __syncthreads();
-        float *part = reinterpret_cast<float *>(ring);       // [256][kPartW]
-        if (warp >= kSmWarp0 && warp < kMmaWarp) {
+        if (ns > 1) {
+            // The cluster's partials: this CTA's rows into the ring's place (its products are
+            // done), then every CTA joins its share of the rows from all of them.
+            named_bar_sync(0, kThr);
+            float *part = reinterpret_cast<float *>(ring);   // [256][kPartW]
             float *p = part + (x * kQT + row) * kPartW;
-            const bool have = alive && nt[x] > 0;
+            const bool have = alive && n > 0;
             p[kKv4Hd] = have ? m : -CUDART_INF_F;
             p[kKv4Hd + 1] = have ? l : 0.f;
 #pragma unroll
@@ -502,33 +506,34 @@ __global__ void __launch_bounds__(kThr, 1)
                         p[32 * c + 8 * g + r + 4] = __uint_as_float(ov[8 * g + 2 * r + 1]) + oc;
                     }
             }
-        }
-        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-        const int per = 2 * kQT / ns, r0 = rank * per;
-        auto cl = cg::this_cluster();
-        for (int i = threadIdx.x; i < per * (kKv4Hd / 4); i += kThr) {
-            const int r = r0 + i / (kKv4Hd / 4), d = 4 * (i % (kKv4Hd / 4)), c = col0 + r;
-            if (c >= total) continue;
-            float mm = -CUDART_INF_F;
-            for (int k = 0; k < ns; ++k) mm = fmaxf(mm, cl.map_shared_rank(part, k)[r * kPartW + kKv4Hd]);
-            const float ref = mm == -CUDART_INF_F ? 0.f : mm;
-            float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < ns; ++k) {
-                const float *p = cl.map_shared_rank(part, k) + r * kPartW;
-                const float f = ex2_approx(p[kKv4Hd] - ref);
-                ll = fmaf(p[kKv4Hd + 1], f, ll);
+            cluster_sync_all();
+            const int r0 = 2 * kQT * rank / ns, per = 2 * kQT * (rank + 1) / ns - r0;
+            auto cl = cg::this_cluster();
+            for (int i = threadIdx.x - 32 * kSmWarp0; i < per * (kKv4Hd / 4); i += 2 * kQT) {
+                const int r = r0 + i / (kKv4Hd / 4), d = 4 * (i % (kKv4Hd / 4)), c = col0 + r;
+                if (c >= total) continue;
+                float mm = -CUDART_INF_F;
+                for (int k = 0; k < ns; ++k) mm = fmaxf(mm, cl.map_shared_rank(part, k)[r * kPartW + kKv4Hd]);
+                const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+                float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < ns; ++k) {
+                    const float *pk = cl.map_shared_rank(part, k) + r * kPartW;
+                    const float f = ex2_approx(pk[kKv4Hd] - ref);
+                    ll = fmaf(pk[kKv4Hd + 1], f, ll);
 #pragma unroll
-                for (int z = 0; z < 4; ++z) o[z] = fmaf(p[d + z], f, o[z]);
+                    for (int z = 0; z < 4; ++z) o[z] = fmaf(pk[d + z], f, o[z]);
+                }
+                const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+                uint2 w;
+                w.x = h2_as_u32(__floats2half2_rn(o[0] * inv, o[1] * inv));
+                w.y = h2_as_u32(__floats2half2_rn(o[2] * inv, o[3] * inv));
+                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + s * a.o_slot + (c / group) * a.o_row +
+                                           (kvh * group + c % group) * kKv4Hd + d) = w;
             }
-            const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-            uint2 w;
-            w.x = h2_as_u32(__floats2half2_rn(o[0] * inv, o[1] * inv));
-            w.y = h2_as_u32(__floats2half2_rn(o[2] * inv, o[3] * inv));
-            *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + s * a.o_slot + (c / group) * a.o_row +
-                                       (kvh * group + c % group) * kKv4Hd + d) = w;
+            cluster_sync_all();
         }
-        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     }
+
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -550,8 +555,22 @@ cudaError_t launch_kv4_flash(const Kv4AttnArgs &a, cudaStream_t st) {
     const long long tiles = ((long long)a.rows * group + 2 * kQT - 1) / (2 * kQT);
     const int nblk = (a.c.max_tok + kKv4Blk - 1) / kKv4Blk;
     const long long hb = (long long)nblk * kKv4Block, ctas = tiles * a.c.kv_heads * a.c.slots;
+    // Cluster size.  A CTA costs about 7 us beside its key tiles of 1.7 us each (4 tiles' time),
+    // one of a cluster 16 us (9 tiles'); take the size with the least rounds x time.  Long shares are
+    // cut once more where causal or ragged lengths would leave few rounds unbalanced (2 x 1024 rows,
+    // 16640 keys: 377 us at 1, 349 at 2, 404 at 3).
+    const long long ktiles = (a.c.max_tok + kKT - 1) / kKT;
     int ns = 1;
-    while (ns < kMaxNs && ctas * ns < num_sms() && nblk >= 8 * ns) ns *= 2;
+    long long best = 0;
+    for (int c = 1; c <= kMaxNs; ++c) {
+        const long long rounds = (ctas * c + num_sms() - 1) / num_sms();
+        const long long cost = rounds * (ktiles / c + (c > 1 ? 9 : 4));
+        if (c == 1 || cost < best) {
+            best = cost;
+            ns = c;
+        }
+    }
+    while (ns * 2 <= kMaxNs && ctas * ns < 4LL * num_sms() && ktiles / (ns * 2) >= 64) ns *= 2;
     if (tiles * a.c.kv_heads * ns > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_k(kv4_flash_kernel, dim3((unsigned)(tiles * a.c.kv_heads * ns), (unsigned)a.c.slots), kThr, kSmem, st, ns,
                     a, hb * a.c.kv_heads, hb, group, (int)tiles, ns);

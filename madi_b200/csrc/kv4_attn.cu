@@ -47,7 +47,7 @@ namespace madi {
 namespace {
 
 constexpr int kMaxNs = 16;                     // CTAs of a cluster (above 8: non-portable size)
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 2;                 // a second block in flight; more cost resident warps
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUp24 = 16777216.f;            // 2^24
 
@@ -557,11 +557,8 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
 constexpr int kFlashCols = 32;
 
 template <int NT, int W, typename T>
-cudaError_t launch_stream(const Kv4AttnArgs &a, cudaStream_t st) {
+cudaError_t launch_stream(const Kv4AttnArgs &a, long long tiles, int ns, cudaStream_t st) {
     auto fn = kv4_stream_kernel<NT, W, T>;
-    const int group = a.heads / a.c.kv_heads;
-    const long long cols = (long long)a.rows * group;
-    const long long tiles = (cols + 4 * NT - 1) / (4 * NT);
     const int nblk = (a.c.max_tok + kKv4Blk - 1) / kKv4Blk;
     const long long hb = (long long)nblk * kKv4Block;
     constexpr size_t kMaxSmem = (size_t)W * kMaxStages * kKv4Block + (size_t)(4 * NT + kMaxNs) * kPart * sizeof(float);
@@ -579,23 +576,51 @@ cudaError_t launch_stream(const Kv4AttnArgs &a, cudaStream_t st) {
             return e1;
         }))
         return e;
-    const long long pairs = tiles * a.c.kv_heads * a.c.slots;
-    // Cluster size: split the keys while that gives work to idle SMs and leaves each warp a block.
-    int ns = 1;
-    while (ns < std::min(max_ns, kMaxNs) && pairs * (ns + 1) <= 2LL * num_sms() && nblk >= (ns + 1) * W) ++ns;
-    const int per_warp = (nblk + ns * W - 1) / (ns * W);
-    const int stages = std::max(1, std::min(per_warp, kMaxStages));
+    ns = std::min(ns, max_ns);
+    const int stages = nblk > ns * W ? kMaxStages : 1;
     const size_t smem = (size_t)W * stages * kKv4Block +
                         (ns > 1 ? (size_t)((4 * NT + ns - 1) / ns) * ns * kPart * sizeof(float) : 0);
     if (tiles * ns > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_k(fn, dim3((unsigned)(tiles * ns), (unsigned)a.c.kv_heads, (unsigned)a.c.slots), 32 * W, smem, st, ns, a,
-                    hb * a.c.kv_heads, hb, group, ns, stages);
+                    hb * a.c.kv_heads, hb, a.heads / a.c.kv_heads, ns, stages);
+}
+
+// Warps per (slot, kv head, tile), in CTAs of 4 or 8: as many as the SMs hold at once (16 a SM with one
+// column group, else 8), none without a block; twice that where each would still have six blocks or
+// more (ragged lengths leave warps idle).  CTAs of 8 where they give more warps, and on a tie unless a
+// short cache has to be cut up finely.  Measured (us): 8 slots x 20 heads x 1500 keys 8.1 as 3 CTAs of 4
+// (8.9 as 1 of 8, 10.3 as 6 of 4), 16 x 20 x 448 ragged 5.7 as 1 of 4 (6.2 as 1 of 8), 8 x 8 x 6000
+// 10.2 as 4 of 8 (10.5 as 8 of 4), 1 x 20 x 1500 4.3 as 6 of 4 (4.7 as 3 of 8), 4 x 8 x 65003 ragged
+// 28.9 as 16 of 8 (32.9 as 8 of 8).
+template <int NT, typename T>
+cudaError_t launch_stream_n(const Kv4AttnArgs &a, long long cols, cudaStream_t st) {
+    const long long tiles = (cols + 4 * NT - 1) / (4 * NT), pairs = tiles * a.c.kv_heads * a.c.slots;
+    const int nblk = (a.c.max_tok + kKv4Blk - 1) / kKv4Blk;
+    long long room = std::max<long long>((NT == 1 ? 16LL : 8LL) * num_sms() / pairs, 1);
+    if (nblk >= 12 * room) room *= 2;
+    const bool cut = nblk <= room;                       // a block per warp
+    auto ctas = [&](int w) {
+        // whole powers of two, or three times one: other cluster sizes pack badly (64 pairs, 48 blocks:
+        // 8.1 us as 4 CTAs of 8, 11.2 as 9 of 4)
+        const long long n = std::min<long long>((nblk + w - 1) / w, room / w);
+        int c = 1;
+        for (int i = 2; i <= kMaxNs; ++i)
+            if (n >= i && ((i & (i - 1)) == 0 || i == 3 || i == 6 || i == 12)) c = i;
+        return c;
+    };
+    const int n4 = ctas(4);
+    if constexpr (NT < 4) {
+        const int n8 = ctas(8);
+        if (room >= 8 && (8 * n8 > 4 * n4 || (8 * n8 == 4 * n4 && (n8 == 1 || !cut))))
+            return launch_stream<NT, 8, T>(a, tiles, n8, st);
+    }
+    return launch_stream<NT, 4, T>(a, tiles, n4, st);
 }
 
 template <typename T>
 cudaError_t launch_stream_t(const Kv4AttnArgs &a, long long cols, cudaStream_t st) {
-    return cols <= 4 ? launch_stream<1, 8, T>(a, st)
-                     : cols <= 8 ? launch_stream<2, 8, T>(a, st) : launch_stream<4, 4, T>(a, st);
+    return cols <= 4 ? launch_stream_n<1, T>(a, cols, st)
+                     : cols <= 8 ? launch_stream_n<2, T>(a, cols, st) : launch_stream_n<4, T>(a, cols, st);
 }
 
 }  // namespace

@@ -27,6 +27,11 @@ the logit filter and suppress list on the shard's columns for every row
 rows); an all-gather of the per-row (max, index, exp sum) parts; and the merge
 (madi_merge_shard_tail) that writes every row's token.  The exchange is a callable
 (out, inp) -> all-gather; NCCL's all_gather_into_tensor by default.
+
+K/V caches in 4 bits (kv4_cache=True): 36 bytes per token and head instead of 256 (self) and 128
+(cross), K and V each.  The QKV projection leaves the new rows in a one-row buffer, kv4.store
+quantises them into the cache at the slot's position, and both attentions read the 4-bit
+caches (kv4.attn); the cross K / V are quantised once per audio chunk.
 """
 from dataclasses import dataclass
 from typing import Callable, List, Optional, Tuple
@@ -34,7 +39,7 @@ from typing import Callable, List, Optional, Tuple
 import numpy as np
 import torch
 
-from . import attn, greedy, q8, shard, synth
+from . import attn, greedy, kv4, q8, shard, synth
 
 D, F, V, HEADS, LAYERS, MAX_TOK, ENC = 1280, 5120, 51866, 20, 4, 448, 1500
 EPS = 1e-5
@@ -120,7 +125,7 @@ class Decoder:
 
     def __init__(self, w: dict, slots: int, device="cuda", act16: bool = False,
                  split: Optional[Tuple[int, int]] = None,
-                 exchange: Optional[Callable[[torch.Tensor, torch.Tensor], None]] = None):
+                 exchange: Optional[Callable[[torch.Tensor, torch.Tensor], None]] = None, kv4_cache: bool = False):
         """act16: the projections take their f32 activations rounded to f16, as the
         reference's batched decode (decodeBlockBatched, decoder.zig:337-341) converts
         them; False keeps the single-token GEMV family's f32 activations.  With act16
@@ -128,7 +133,8 @@ class Decoder:
         the producer), so the projections stage half the activation bytes.
         split: (world, rank) for the column-split vocab head (see the module
         docstring); exchange(out, inp): all-gather of inp from every rank into out,
-        rank-major (default: torch.distributed.all_gather_into_tensor)."""
+        rank-major (default: torch.distributed.all_gather_into_tensor).
+        kv4_cache: keep the self and cross K / V in 4 bits (see the module docstring)."""
         if not 1 <= slots <= 16:
             raise ValueError("1..16 token slots")
         if split is not None and not (split[0] >= 1 and 0 <= split[1] < split[0]):
@@ -154,8 +160,17 @@ class Decoder:
         self.x, self.q, self.ao, self.mo = (torch.zeros((S, D), **f32) for _ in range(4))
         self.xb = torch.zeros((S, D), **act)
         self.mh = torch.zeros((S, F), **act)
-        self.kc = [torch.zeros((S, MAX_TOK, D), **f32) for _ in range(LAYERS)]
-        self.vc = [torch.zeros((S, MAX_TOK, D), **f32) for _ in range(LAYERS)]
+        self.kv4_cache = kv4_cache
+        if kv4_cache:
+            self.self4 = [kv4.Cache.empty(S, HEADS, MAX_TOK, device) for _ in range(LAYERS)]
+            self.cross4 = [None] * LAYERS
+            # a token's K and V rows before they are quantised (shared by the layers): a cache of one row
+            self.kc = [torch.zeros((S, 1, D), **f32)] * LAYERS
+            self.vc = [torch.zeros((S, 1, D), **f32)] * LAYERS
+            self.row0 = torch.zeros(S, dtype=torch.int32, device=device)
+        else:
+            self.kc = [torch.zeros((S, MAX_TOK, D), **f32) for _ in range(LAYERS)]
+            self.vc = [torch.zeros((S, MAX_TOK, D), **f32) for _ in range(LAYERS)]
         self.ck = [None] * LAYERS
         self.cv = [None] * LAYERS
         self.split = split
@@ -192,6 +207,17 @@ class Decoder:
         stays valid across audio chunks."""
         S, T, _ = enc_states.shape
         flat = enc_states.reshape(S * T, D).contiguous()
+        if self.kv4_cache:
+            if self.ck[0] is None or self.ck[0].shape != (S, T, D):
+                # the projections before they are quantised, shared by the layers
+                self.ck = [torch.empty((S, T, D), dtype=torch.float16, device=flat.device)] * LAYERS
+                self.cv = [torch.empty((S, T, D), dtype=torch.float16, device=flat.device)] * LAYERS
+                self.cross4 = [kv4.Cache.empty(S, HEADS, T, flat.device) for _ in range(LAYERS)]
+            for l, L in enumerate(self.layers):
+                q8.linear(L.ck, flat, out=self.ck[l].view(S * T, D), stream=stream)
+                q8.linear(L.cv, flat, bias=L.cvb, out=self.cv[l].view(S * T, D), stream=stream)
+                kv4.store(self.cross4[l], self.ck[l], self.cv[l], stream=stream)
+            return
         for l, L in enumerate(self.layers):
             if self.ck[l] is None or self.ck[l].shape != (S, T, D):
                 self.ck[l] = torch.empty((S, T, D), dtype=torch.float16, device=flat.device)
@@ -250,12 +276,20 @@ class Decoder:
         greedy.emb_pos_q8(self.emb, self.tokens, self.pos, self.pos_emb, out=self.x, **s)
         for l, L in enumerate(self.layers):
             q8.layer_norm(self.x, *L.aln, eps=EPS, out=self.xb, **s)
-            q8.qkv(L.qkv, self.xb, L.qb, L.vb, self.kc[l], self.vc[l], self.pos, q_out=self.q, **r)
-            attn.self_attn(self.q, self.kc[l], self.vc[l], self.pos, HEADS, out=self.ao, **s)
+            if self.kv4_cache:
+                q8.qkv(L.qkv, self.xb, L.qb, L.vb, self.kc[l], self.vc[l], self.row0, q_out=self.q, **r)
+                kv4.store(self.self4[l], self.kc[l], self.vc[l], pos=self.pos, **s)
+                kv4.attn(self.q, self.self4[l], HEADS, pos=self.pos, out=self.ao, **s)
+            else:
+                q8.qkv(L.qkv, self.xb, L.qb, L.vb, self.kc[l], self.vc[l], self.pos, q_out=self.q, **r)
+                attn.self_attn(self.q, self.kc[l], self.vc[l], self.pos, HEADS, out=self.ao, **s)
             q8.linear(L.o, self.ao, out=self.mo, **r)
             q8.bias_res_ln(self.x, self.mo, L.ob, *L.caln, eps=EPS, out=self.xb, **s)
             q8.linear(L.cq, self.xb, bias=L.cqb, out=self.q, **r)
-            attn.cross_attn(self.q, self.ck[l], self.cv[l], HEADS, out=self.ao, **s)
+            if self.kv4_cache:
+                kv4.attn(self.q, self.cross4[l], HEADS, out=self.ao, **s)
+            else:
+                attn.cross_attn(self.q, self.ck[l], self.cv[l], HEADS, out=self.ao, **s)
             q8.linear(L.co, self.ao, out=self.mo, **r)
             q8.bias_res_ln(self.x, self.mo, L.cob, *L.mln, eps=EPS, out=self.xb, **s)
             q8.linear(L.fc1, self.xb, bias=L.m0b, epi=q8.EPI_BIAS_GELU, out=self.mh, **r)
@@ -267,7 +301,7 @@ class Decoder:
         self K/V rows 0..pos (counted at a full 448-row cache), the cross K/V, the
         head (this rank's shard of it when split)."""
         per_layer = (3 * D * D + 3 * D * D + 2 * F * D) * (1 + 1 / 16)
-        kv_self = 2 * self.slots * MAX_TOK * D * 4
-        kv_cross = 2 * self.slots * ENC * D * 2
+        kv_self = 2 * self.slots * MAX_TOK * (HEADS * 36 if self.kv4_cache else D * 4)
+        kv_cross = 2 * self.slots * ENC * (HEADS * 36 if self.kv4_cache else D * 2)
         head = (V if self.split is None else self.h1 - self.h0) * D * (1 + 1 / 16)
         return int(LAYERS * (per_layer + kv_self + kv_cross) + head)

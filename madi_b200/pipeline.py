@@ -41,7 +41,7 @@ def synthetic_mel(chunks: int, first: int = 0) -> np.ndarray:
 class Transcriber:
     def __init__(self, slots: int = 8, enc_layers: int = 32, tokens: int = 224, seed: int = 1, device="cuda",
                  split: Optional[Tuple[int, int]] = None, act16: Optional[bool] = None,
-                 decoders: Optional[int] = None, exchange: str = "auto"):
+                 decoders: Optional[int] = None, exchange: str = "auto", kv4_cache: bool = False):
         """split: (world, rank) -- the decoder's vocab head column-split over the
         ranks of the default process group (one process per GPU), its logits
         exchanged by all-gathers inside the captured token step (see `exchange`).  Every rank
@@ -58,7 +58,8 @@ class Transcriber:
         exchange: how the split head's all-gathers travel -- "nccl" (torch.distributed
         all_gather_into_tensor), "p2p" (madi_b200.p2p.PeerExchange: one kernel storing
         into the peers' memory over NVLink; ranks on distinct GPUs), or "auto" (the
-        default: p2p when the ranks sit on distinct GPUs, else nccl)."""
+        default: p2p when the ranks sit on distinct GPUs, else nccl).
+        kv4_cache: the decoders keep their K / V caches in 4 bits (decoder.Decoder)."""
         if tokens < 1 or tokens + 1 > dec.MAX_TOK:
             raise ValueError(f"1..{dec.MAX_TOK - 1} tokens per chunk")
         self.encoder = enc.Encoder(enc_layers, seed, device)
@@ -91,7 +92,8 @@ class Transcriber:
                 exchanges = [(lambda g: (lambda out, inp: dist.all_gather_into_tensor(out, inp, group=g)))(g)
                              for g in self.groups]
             self.exchange = exchange
-        self.decoders = [dec.Decoder(w, slots, device, act16=act16, split=split, exchange=exchanges[i])
+        self.decoders = [dec.Decoder(w, slots, device, act16=act16, split=split, exchange=exchanges[i],
+                                     kv4_cache=kv4_cache)
                          for i in range(decoders)]
         self.decoder = self.decoders[0]
         self.split = split

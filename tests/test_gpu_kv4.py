@@ -202,3 +202,179 @@ def test_nan_rows_reach_only_the_queries_that_attend_them(madi):
             p0 = bad - 2
             o = _host(kv4.attn(q, c, H, pos=_u32([p0])))[0].reshape(T, H, 64)
             assert np.isfinite(o[:, 0]).all() and np.isfinite(o[:2, 1]).all() and np.isnan(o[2:, 1]).all()
+
+
+def _rand_store(slots, heads, max_tok, seed):
+    import torch
+    from madi_b200 import kv4
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    c = kv4.Cache.empty(slots, heads, max_tok)
+    k, v = (torch.randn((slots, max_tok, heads * 64), generator=g, device="cuda") for _ in range(2))
+    return c, k, v, g
+
+
+@pytest.mark.parametrize("dt,rows,heads,kv_heads,max_tok", [
+    (F32, 1, 4, 4, 320), (F16, 1, 8, 2, 9000), (F32, 6, 4, 4, 700), (F16, 40, 4, 2, 400), (F16, 40, 2, 2, 20000)])
+def test_captured_calls_on_another_stream(madi, dt, rows, heads, kv_heads, max_tok):
+    """Store, attention and load captured on a side stream, two graphs of them replayed at once on
+    two streams with inputs that change between replays, against eager calls on the default stream;
+    lengths are read on the device."""
+    import torch
+    from madi_b200 import kv4
+    tdt = torch.float32 if dt == F32 else torch.float16
+    S = 2
+    jobs = []
+    for j in range(2):
+        c, k, v, g = _rand_store(S, kv_heads, max_tok, 10 + j)
+        q = torch.randn((S, rows, heads * 64), generator=g, device="cuda").to(tdt)
+        pos = torch.tensor([max_tok - rows, 5], dtype=torch.int32, device="cuda")
+        out = torch.zeros_like(q)
+        ko, vo = (torch.zeros((S, 3, kv_heads * 64), device="cuda") for _ in range(2))
+        st = torch.cuda.Stream()
+
+        def call(c=c, k=k, v=v, q=q, pos=pos, out=out, ko=ko, vo=vo, stream=None):
+            kv4.store(c, k, v, stream=stream)
+            kv4.attn(q, c, heads, pos=pos, out=out, stream=stream)
+            kv4.load(c, 3, pos=pos, k_out=ko, v_out=vo, stream=stream)
+        call()                                              # one-time set-up
+        torch.cuda.synchronize()
+        g2 = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g2, stream=st):
+            call()
+        jobs.append((call, g2, st, (k, v, q, pos), (out, ko, vo), c))
+    for turn in range(3):
+        wants = []
+        for call, g2, st, (k, v, q, pos), outs, c in jobs:
+            k.normal_()
+            v.normal_()
+            q.copy_(torch.randn(q.shape, device="cuda"))
+            pos.copy_(torch.tensor([(max_tok - rows) // (turn + 1), 7 * turn], dtype=torch.int32))
+            for o in outs:                                  # rows that load leaves alone are compared too
+                o.fill_(-1.0)
+            call()
+            torch.cuda.synchronize()
+            wants.append([o.clone() for o in outs])
+            for o in outs:
+                o.fill_(-1.0)
+            c.data.fill_(0xFF)
+        torch.cuda.synchronize()
+        for _, g2, st, _, _, _ in jobs:
+            with torch.cuda.stream(st):
+                g2.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, _, outs, _), want in zip(jobs, wants):
+            for o, w in zip(outs, want):
+                assert torch.equal(o, w)
+        # and eagerly on a stream that is not the current one
+        call, _, st, _, outs, c = jobs[0]
+        for o in outs:
+            o.fill_(-1.0)
+        st.wait_stream(torch.cuda.current_stream())
+        call(stream=st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants[0]))
+
+
+def test_row_by_row_append_equals_one_store(madi):
+    import torch
+    from madi_b200 import kv4
+    c, k, v, _ = _rand_store(3, 2, 150, 4)
+    kv4.store(c, k, v)
+    d = kv4.Cache.empty(3, 2, 150)
+    for i in range(150):
+        kv4.store(d, k[:, i:i + 1], v[:, i:i + 1], pos=torch.full((3,), i, dtype=torch.int32, device="cuda"))
+    a, b = kv4.load(c, 150, dtype=torch.float32), kv4.load(d, 150, dtype=torch.float32)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dt", [F32, F16])
+def test_rows_give_the_same_as_one_by_one(madi, dt):
+    """A causal call of several rows against one call per row: both within the bound of the exact
+    result; checked here to the type's rounding of each other."""
+    import torch
+    from madi_b200 import kv4
+    tdt = torch.float32 if dt == F32 else torch.float16
+    c, k, v, g = _rand_store(2, 2, 300, 6)
+    kv4.store(c, k, v)
+    q = torch.randn((2, 20, 4 * 64), generator=g, device="cuda").to(tdt)
+    p0 = torch.tensor([250, 0], dtype=torch.int32, device="cuda")
+    many = kv4.attn(q, c, 4, pos=p0)
+    one = torch.stack([kv4.attn(q[:, i].contiguous(), c, 4, pos=p0 + i) for i in range(20)], 1)
+    torch.cuda.synchronize()
+    # f32: each call is within 2e-6 of the largest output (its sums in another order); f16: the weights'
+    # rounding in one of the two (2^-11 of sum p|v| <= max|v| there), and both outputs' own (2^-11)
+    tol = 4e-6 * many.abs().max().item() if dt == F32 else 4 * 2.0 ** -11 * v.abs().max().item()
+    assert (many.double() - one.double()).abs().max().item() <= tol
+
+
+def test_f32_results_are_as_exact_as_f32_arithmetic(madi):
+    """In norm: a plain f32 form of these sizes is 2e-7 to 5e-7 off the 64-bit result (its sums of 64
+    products and of up to 1500 weights round at 2^-24 each); 1e-6 leaves a factor of two."""
+    import torch
+    from madi_b200 import kv4
+    for slots, rows, heads, kv_heads, max_tok in ((2, 1, 4, 4, 1500), (1, 5, 4, 4, 448), (1, 3, 6, 2, 900)):
+        g = np.random.default_rng(max_tok)
+        data = R.random_cache(g, slots, kv_heads, max_tok, [max_tok] * slots)
+        q = (g.standard_normal((slots, rows, heads * 64)) * 1.5).astype(F32)
+        want, _ = R.attend(q, data, max_tok, heads, R.key_counts(slots, rows, max_tok))
+        got = _host(kv4.attn(_t(q), _cache(data, max_tok), heads)).astype(np.float64)
+        assert np.linalg.norm(got - want) <= 1e-6 * np.linalg.norm(want)
+
+
+def test_offsets_past_32_bits(madi):
+    """A cache of more than 2^32 bytes: rows stored at its end are the ones attended and read."""
+    import torch
+    from madi_b200 import kv4
+    heads, max_tok = 8, 1 << 20
+    slots = 8
+    c = kv4.Cache.empty(slots, heads, max_tok)
+    assert c.data.numel() > 1 << 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    k, v = (torch.randn((slots, 64, heads * 64), generator=g, device="cuda") for _ in range(2))
+    at = torch.full((slots,), max_tok - 64, dtype=torch.int32, device="cuda")
+    kv4.store(c, k, v, pos=at)
+    ko, vo = kv4.load(c, 64, pos=at, dtype=torch.float32)
+    small = kv4.Cache.empty(slots, heads, 64)
+    kv4.store(small, k, v)
+    ks, vs = kv4.load(small, 64, dtype=torch.float32)
+    assert torch.equal(ko, ks) and torch.equal(vo, vs)
+    # attention over the last slot's last block: all other rows hold keys that no query can prefer
+    c.data.zero_()                                          # codes 0, c = d = 0: scores 0, values 0
+    kv4.store(c, k, v, pos=at)
+    big = 50.0 * k[:, 63].reshape(slots, heads, 64)         # each query looks for its own last key
+    for dt, rows in ((torch.float32, 1), (torch.float16, 33)):
+        q = big.reshape(slots, 1, heads * 64).expand(slots, rows, heads * 64).contiguous().to(dt)
+        o = kv4.attn(q, c, heads)
+        s = kv4.attn(q, small, heads)
+        torch.cuda.synchronize()
+        # 2^20 keys of score 0 against scores of some hundreds: their weights vanish
+        assert (o.float() - s.float()).abs().max().item() <= 1e-3
+
+
+def test_refusals_on_the_device(madi):
+    import torch
+    from madi_b200 import kv4
+    from madi_b200._lib import MadiError
+    c, k, v, _ = _rand_store(2, 2, 70, 1)
+    q = torch.zeros((2, 1, 256), device="cuda")
+    before = c.data.clone()
+    bad = [lambda: kv4.store(c, k[:, 1:, :].reshape(-1)[1:1 + 2 * 60 * 128].view(2, 60, 128), v[:, :60]),      # strides differ
+           lambda: kv4.attn(q, c, 4, out=q),                                        # in place
+           lambda: kv4.attn(torch.zeros((2, 1, 3 * 64), device="cuda"), c, 3),      # 3 heads over 2 kv heads
+           lambda: kv4.attn(q, c, 4, pos=torch.zeros(2, dtype=torch.int32)),        # a host index
+           lambda: kv4.attn(q.cpu(), c, 4),
+           lambda: kv4.store(c, k[:1].expand(2, -1, -1), v[:1].expand(2, -1, -1)),  # overlapping slots
+           lambda: kv4.load(c, 70, k_out=k, v_out=k)]
+    wide = torch.zeros((2, 3, 130), device="cuda")
+    bad.append(lambda: kv4.store(c, wide[..., 1:129], wide[..., 1:129]))            # rows not 16-byte aligned
+    for i, f in enumerate(bad):
+        with pytest.raises((ValueError, MadiError)):
+            f()
+    torch.cuda.synchronize()
+    assert torch.equal(c.data, before)
+    # nothing to do
+    kv4.store(c, k[:, :0], v[:, :0])
+    assert kv4.load(c, 0)[0].shape == (2, 0, 128)
+    assert kv4.attn(q[:, :0], c, 4).shape == (2, 0, 256)

@@ -74,7 +74,7 @@ def _index(t: Optional[torch.Tensor], name: str, c: Cache) -> int:
     """Device pointer of a per-slot u32 / int32 vector (0: not given)."""
     if t is None:
         return 0
-    if t.dtype not in _U32 or t.shape != (c.slots,) or not t.is_contiguous():
+    if t.dtype not in _U32 or t.dim() != 1 or t.numel() != c.slots or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous u32 or int32 [{c.slots}] tensor")
     if t.get_device() != c.device:
         raise ValueError(f"{name} is on {t.device}, the cache on {c.data.device}")
@@ -104,7 +104,9 @@ def _pair(k: torch.Tensor, v: torch.Tensor, names: str, c: Cache) -> Tuple[int, 
     lay = _layout(k, names, c, c.kv_heads * HEAD_DIM)
     if k.dim() != 3:
         raise ValueError(f"{names} must be a [slots][rows][kv_heads * 64] tensor")
-    if v.shape != k.shape or v.dtype != k.dtype or _layout(v, "v" + names[1:], c, c.kv_heads * HEAD_DIM) != lay:
+    if v.shape != k.shape or v.dtype != k.dtype or (
+            (v.stride() != k.stride() or v.get_device() != c.device) and
+            _layout(v, "v" + names[1:], c, c.kv_heads * HEAD_DIM) != lay):
         raise ValueError(f"v{names[1:]} must match {names} in shape, type and strides")
     return lay
 
@@ -163,7 +165,10 @@ def attn(q: torch.Tensor, cache: Cache, heads: int, pos: Optional[torch.Tensor] 
             out = (torch.empty if n is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape and type")
-    _, o_slot, o_row = _layout(out, "out", cache, heads * HEAD_DIM)
+    if out.stride() == q.stride() and out.get_device() == cache.device:
+        o_slot, o_row = q_slot, q_row
+    else:
+        _, o_slot, o_row = _layout(out, "out", cache, heads * HEAD_DIM)
     rc = _lib.load().madi_kv4_attn(cache._struct, _QUERY(q.data_ptr(), out.data_ptr(), *args, q_slot, q_row, o_slot,
                                                          o_row, _DT[q.dtype], heads, rows, 0),
                                    _raw_stream(stream, cache))

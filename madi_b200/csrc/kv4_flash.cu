@@ -9,14 +9,14 @@
 // f16 parts, the values' c as one more column of V, beside a column of ones that gives the sum of
 // the weights.  Rounding c + d n' to f16 instead would add two more errors of the output's own size.
 //
-// One CTA per (256 query columns of one kv head, slot, share of the keys); a column is one
+// One CTA per (128 or 256 query columns of one kv head, slot, share of the keys); a column is one
 // (query row, query head of the kv head).  Warps:
 //   warps 0-2   read the packed K and V rows (32 bytes and (c, d) each), write the f16 rows and the
-//               c's into a 3-stage ring, in the SWIZZLE_128B layout; the next tile's bytes are in
+//               c's into a ring of stages, in the SWIZZLE_128B layout; the next tile's bytes are in
 //               flight meanwhile;
 //   warp 3      issues the products (S: 5 steps, both operands in shared memory; O: P in TMEM as
 //               the first operand, V N-contiguous) and owns TMEM;
-//   warps 4-11  the softmax of the two 128-column tiles (thread = column = TMEM lane), as in
+//   warps 4-11  (4-7) the softmax of the 128-column tiles (thread = column = TMEM lane), as in
 //               flash_enc.cu: S in TMEM, P written back as f16, O rescaled when a maximum grew.
 // Within every 8 dims the shared-memory order is 0 4 1 5 2 6 3 7 -- what one mask of a code word
 // gives as a pair of f16 -- for Q and K alike, and for V's columns, which are put back in order
@@ -44,14 +44,11 @@ namespace {
 
 constexpr int kQT = 128;                       // query columns per tile
 constexpr int kKT = 96;                        // keys per tile: S, P and O of two tiles fit TMEM, a row of S registers
-constexpr int kNS = 3;                         // ring stages
 constexpr int kTile = 128 * 64 * 2;            // bytes of one [128][64] f16 tile (Q)
 constexpr int kKTile = kKT * 64 * 2;           // bytes of one [96][64] f16 tile (K, V)
 constexpr int kDeqThr = 96;                    // warps 0..2
 constexpr int kMmaWarp = 3;
 constexpr int kSmWarp0 = 4;                    // warps 4..7: tile 0; 8..11: tile 1
-constexpr int kThr = 32 * 12;
-constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTileCols = 256, kPCol = 96, kOCol = 144, kSumCol = kOCol + kKv4Hd;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kIdescS = idesc_f16_f32(kQT, kKT);
@@ -60,23 +57,30 @@ constexpr int kMaxNs = 8;
 constexpr float kSlack = 8.f;                  // base-2 head room of the softmax reference
 constexpr int kPartW = kKv4Hd + 2;             // a row's partial: O, m, l
 
-struct __align__(16) FlashShared {
-    uint64_t q_full;         // 256: both Q tiles and their sums written
+template <int kX, int kNS> struct __align__(16) FlashShared {
+    uint64_t q_full;         // kX * 128: the Q tiles and their sums written
     uint64_t kv_full[kNS];   // 96: a stage's keys and values written
     uint64_t kv_empty[kNS];  // its products complete
-    uint64_t s_full[2], s_free[2], p_ready[2], o_done[2];
+    uint64_t s_full[kX], s_free[kX], p_ready[kX], o_done[kX];
     uint64_t drain;
     uint32_t tmem_base;
     int abort;
 };
 
-// Q tiles 0 and 1 | sums of Q (tile x in 16-byte chunks 2x, 2x + 1 of each row) | stages of
-// K | V | a key's extra columns, in one row: chunks 0, 1 the columns 64.. of V (the value's c, then
-// 1: their products with P are sum p c and sum p), chunks 2, 3 the fifth step of K (c twice).
-constexpr size_t kQBytes = 3 * (size_t)kTile, kStage = 3 * (size_t)kKTile;
-constexpr size_t kSmem = 1024 + kQBytes + kNS * kStage + sizeof(FlashShared);
-static_assert(kSmem <= 227 * 1024, "shared memory");
-static_assert(kNS * kStage >= 2 * kQT * kPartW * sizeof(float), "the partials take the ring's place");
+// A CTA with kX query tiles: two with a ring of three stages, one CTA per SM; or one with two stages,
+// two CTAs per SM.  Shared memory: Q tiles | sums of Q (tile x in 16-byte chunks 2x, 2x + 1 of each row)
+// | stages of K | V | a key's extra columns, in one row: chunks 0, 1 the columns 64.. of V (the value's
+// c, then 1: their products with P are sum p c and sum p), chunks 2, 3 the fifth step of K (c twice).
+constexpr size_t kStage = 3 * (size_t)kKTile;
+template <int kX> struct FlashCfg {
+    static constexpr int kNS = kX == 2 ? 3 : 2, kPerSm = kX == 2 ? 1 : 2, kThr = 32 * (4 + 4 * kX);
+    static constexpr uint32_t kTmemCols = 256 * kX;
+    using Shared = FlashShared<kX, kNS>;
+    static constexpr size_t kQBytes = (kX + 1) * (size_t)kTile;
+    static constexpr size_t kSmem = 1024 + kQBytes + kNS * kStage + sizeof(Shared);
+    static_assert(kPerSm * (kSmem + 1024) <= 227 * 1024, "shared memory");
+    static_assert(kNS * kStage >= kX * kQT * kPartW * sizeof(float), "the partials take the ring's place");
+};
 
 MADI_DEV void wait_drain(uint64_t *bar, uint32_t parity) {
     const long long t0 = clock64();
@@ -131,24 +135,29 @@ struct RowBytes {
     uint32_t cd;
 };
 
-__global__ void __launch_bounds__(kThr, 1)
+template <int kX>
+__global__ void __launch_bounds__(FlashCfg<kX>::kThr, FlashCfg<kX>::kPerSm)
     kv4_flash_kernel(const Kv4AttnArgs a, long long slot_bytes, long long head_bytes, int group, int tiles, int ns) {
+    using Cfg = FlashCfg<kX>;
+    using Shared = typename Cfg::Shared;
+    constexpr int kNS = Cfg::kNS, kThr = Cfg::kThr;
+    constexpr size_t kQBytes = Cfg::kQBytes;
     extern __shared__ uint8_t kv4f_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kv4f_smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *qs = smem, *qx = smem + 2 * kTile, *ring = smem + kQBytes;
-    FlashShared *sh = reinterpret_cast<FlashShared *>(ring + kNS * kStage);
+    uint8_t *qs = smem, *qx = smem + kX * kTile, *ring = smem + kQBytes;
+    Shared *sh = reinterpret_cast<Shared *>(ring + kNS * kStage);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % ns;
     // causal rows: the last tiles have the most keys, so they start first
     const int tile = tiles - 1 - (int)(blockIdx.x / ns) % tiles, kvh = (int)(blockIdx.x / ns) / tiles, s = blockIdx.y;
     pdl_trigger();
     if (threadIdx.x == 0) {
-        mbar_init(&sh->q_full, 2 * kQT);
+        mbar_init(&sh->q_full, kX * kQT);
         for (int i = 0; i < kNS; ++i) {
             mbar_init(&sh->kv_full[i], kDeqThr);
             mbar_init(&sh->kv_empty[i], 1);
         }
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < kX; ++x) {
             mbar_init(&sh->s_full[x], 1);
             mbar_init(&sh->s_free[x], kQT);
             mbar_init(&sh->p_ready[x], kQT);
@@ -159,23 +168,27 @@ __global__ void __launch_bounds__(kThr, 1)
         fence_mbar_init();
     }
     pdl_wait();
-    const int total = kv4_rows(a.n, s, a.rows) * group, col0 = tile * 2 * kQT;
+    const int total = kv4_rows(a.n, s, a.rows) * group, col0 = tile * kX * kQT;
     if (col0 >= total) return;                               // padding only (the whole cluster leaves)
     // key tiles of column tile x in this CTA's share [j0, j1)
-    int top[2], nt[2];
+    int top[kX], nt[kX], kmax = 0, nmax = 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < kX; ++x) {
         const int last = min(col0 + (x + 1) * kQT, total) - 1;
         top[x] = last >= col0 + x * kQT ? kv4_keys(a.pos, a.lens, s, last / group, a.c.max_tok) : 0;
     }
-    const int kmax = max(top[0], top[1]), all = (kmax + kKT - 1) / kKT;
+#pragma unroll
+    for (int x = 0; x < kX; ++x) kmax = max(kmax, top[x]);
+    const int all = (kmax + kKT - 1) / kKT;
     const int j0 = (int)((long long)all * rank / ns), j1 = (int)((long long)all * (rank + 1) / ns);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) nt[x] = max(min((top[x] + kKT - 1) / kKT, j1) - j0, 0);
-    const int nmax = max(nt[0], nt[1]);
+    for (int x = 0; x < kX; ++x) {
+        nt[x] = max(min((top[x] + kKT - 1) / kKT, j1) - j0, 0);
+        nmax = max(nmax, nt[x]);
+    }
 
     if (warp == kMmaWarp) {
-        tmem_alloc(&sh->tmem_base, kTmemCols);
+        tmem_alloc(&sh->tmem_base, Cfg::kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -265,11 +278,11 @@ __global__ void __launch_bounds__(kThr, 1)
                 umma_commit(&sh->s_full[y]);
                 return true;
             };
-            for (int y = 0; ok && y < 2; ++y)
+            for (int y = 0; ok && y < kX; ++y)
                 if (nt[y] > 0) ok = issue_s(y, 0);
             for (int j = 0; ok && j < nmax; ++j) {
                 const int st = j % kNS;
-                for (int y = 0; ok && y < 2; ++y) {
+                for (int y = 0; ok && y < kX; ++y) {
                     if (j >= nt[y]) continue;
                     if (j + 1 < nt[y] &&
                         (!mbar_wait(&sh->s_free[y], (uint32_t)j & 1u, abort_flag, a.dev_err) || !issue_s(y, j + 1))) {
@@ -302,7 +315,7 @@ __global__ void __launch_bounds__(kThr, 1)
     } else {
         // ------------------------------------------------ softmax, one query column per thread
         float m = -CUDART_INF_F;
-        const int x = warp >= kSmWarp0 + 4 ? 1 : 0;          // column tile of this warp
+        const int x = (warp - kSmWarp0) >> 2;                // column tile of this warp
         const int row = (warp & 3) * 32 + lane;              // column within the tile
         const uint32_t tb = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kTileCols;
         const int col = col0 + x * kQT + row;
@@ -507,9 +520,9 @@ __global__ void __launch_bounds__(kThr, 1)
                     }
             }
             cluster_sync_all();
-            const int r0 = 2 * kQT * rank / ns, per = 2 * kQT * (rank + 1) / ns - r0;
+            const int r0 = kX * kQT * rank / ns, per = kX * kQT * (rank + 1) / ns - r0;
             auto cl = cg::this_cluster();
-            for (int i = threadIdx.x - 32 * kSmWarp0; i < per * (kKv4Hd / 4); i += 2 * kQT) {
+            for (int i = threadIdx.x - 32 * kSmWarp0; i < per * (kKv4Hd / 4); i += kX * kQT) {
                 const int r = r0 + i / (kKv4Hd / 4), d = 4 * (i % (kKv4Hd / 4)), c = col0 + r;
                 if (c >= total) continue;
                 float mm = -CUDART_INF_F;
@@ -538,42 +551,52 @@ __global__ void __launch_bounds__(kThr, 1)
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, kTmemCols);
+        tmem_dealloc(tmem, Cfg::kTmemCols);
     }
 }
 
-}  // namespace
-
-cudaError_t launch_kv4_flash(const Kv4AttnArgs &a, cudaStream_t st) {
+template <int kX>
+cudaError_t launch_flash(const Kv4AttnArgs &a, cudaStream_t st) {
+    using Cfg = FlashCfg<kX>;
     static std::once_flag once;
     static cudaError_t once_status;
     if (cudaError_t e = run_once(once, once_status, [] {
-            return cudaFuncSetAttribute(kv4_flash_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+            return cudaFuncSetAttribute(kv4_flash_kernel<kX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmem);
         }))
         return e;
     const int group = a.heads / a.c.kv_heads;
-    const long long tiles = ((long long)a.rows * group + 2 * kQT - 1) / (2 * kQT);
+    const long long tiles = ((long long)a.rows * group + kX * kQT - 1) / (kX * kQT);
     const int nblk = (a.c.max_tok + kKv4Blk - 1) / kKv4Blk;
     const long long hb = (long long)nblk * kKv4Block, ctas = tiles * a.c.kv_heads * a.c.slots;
+    const long long room = (long long)num_sms() * Cfg::kPerSm;
     // Cluster size.  A CTA costs about 7 us beside its key tiles of 1.7 us each (4 tiles' time),
     // one of a cluster 16 us (9 tiles'); take the size with the least rounds x time.  Long shares are
-    // cut once more where causal or ragged lengths would leave few rounds unbalanced (2 x 1024 rows,
-    // 16640 keys: 377 us at 1, 349 at 2, 404 at 3).
+    // cut once more where causal or ragged lengths would leave few rounds unbalanced (2 x 1024 rows x
+    // 32 heads, 16640 keys: 377 us at 1, 349 at 2, 404 at 3).
     const long long ktiles = (a.c.max_tok + kKT - 1) / kKT;
     int ns = 1;
     long long best = 0;
     for (int c = 1; c <= kMaxNs; ++c) {
-        const long long rounds = (ctas * c + num_sms() - 1) / num_sms();
+        const long long rounds = (ctas * c + room - 1) / room;
         const long long cost = rounds * (ktiles / c + (c > 1 ? 9 : 4));
         if (c == 1 || cost < best) {
             best = cost;
             ns = c;
         }
     }
-    while (ns * 2 <= kMaxNs && ctas * ns < 4LL * num_sms() && ktiles / (ns * 2) >= 64) ns *= 2;
+    while (ns * 2 <= kMaxNs && ctas * ns < 4 * room && ktiles / (ns * 2) >= 64) ns *= 2;
     if (tiles * a.c.kv_heads * ns > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_k(kv4_flash_kernel, dim3((unsigned)(tiles * a.c.kv_heads * ns), (unsigned)a.c.slots), kThr, kSmem, st, ns,
-                    a, hb * a.c.kv_heads, hb, group, (int)tiles, ns);
+    return launch_k(kv4_flash_kernel<kX>, dim3((unsigned)(tiles * a.c.kv_heads * ns), (unsigned)a.c.slots), Cfg::kThr,
+                    Cfg::kSmem, st, ns, a, hb * a.c.kv_heads, hb, group, (int)tiles, ns);
+}
+
+}  // namespace
+
+// One query tile per CTA where the columns fit one (8 slots x 20 heads x 1500 keys: 64 columns 34 us, with
+// two 43; 128: 36, 44), else two, which share the keys they unpack (2 x 1024 rows x 32 heads, 16640 keys:
+// 349 us, with one 363).
+cudaError_t launch_kv4_flash(const Kv4AttnArgs &a, cudaStream_t st) {
+    return (long long)a.rows * (a.heads / a.c.kv_heads) <= kQT ? launch_flash<1>(a, st) : launch_flash<2>(a, st);
 }
 
 }  // namespace madi

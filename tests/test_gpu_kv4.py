@@ -158,7 +158,9 @@ def test_attn_one_token(madi, slots, heads, kv_heads, max_tok, lens, dt):
     (2, 5, 4, 4, 448, [0, 443], None, None), (2, 5, 4, 2, 100, [98, 60], None, [5, 2]),
     (3, 7, 6, 2, 300, None, [0, 65, 300], [7, 7, 0]), (1, 33, 3, 1, 90, [0], None, None),
     (2, 17, 2, 2, 64, None, None, [16, 17]), (1, 130, 2, 1, 700, [500], None, None),
-    (2, 70, 4, 4, 260, [0, 190], None, [70, 41])])
+    (2, 70, 4, 4, 260, [0, 190], None, [70, 41]), (1, 60, 2, 1, 3000, [2900], None, None),
+    (2, 33, 2, 2, 4100, None, [4099, 96], [33, 1]), (1, 140, 2, 1, 5000, [4800], None, [137]),
+    (2, 129, 1, 1, 97, None, [97, 0], None), (1, 300, 1, 1, 1000, [700], None, None)])
 def test_attn_many_tokens(madi, slots, rows, heads, kv_heads, max_tok, pos, lens, n, dt):
     _attn_case(madi, slots, rows, heads, kv_heads, max_tok, dt, pos=pos, lens=lens, n=n)
 

@@ -23,6 +23,7 @@ BLOCK_TOKENS = 64          # tokens per block
 BLOCK_BYTES = 4608         # K and V of a block: codes and (c, d) of each
 _DT = {torch.float32: MADI_F32, torch.float16: MADI_F16}
 _U32 = (torch.int32, torch.uint32)
+_current_device = torch._C._cuda_getDevice
 # the structs of include/madi_q8.h
 _CACHE = struct.Struct("=Qiii4x").pack
 _ROWS = struct.Struct("=QQQQqqii").pack
@@ -58,6 +59,8 @@ class Cache:
 def _raw_stream(stream, c: Cache) -> int:
     if c.device < 0:
         raise ValueError("the cache is in host memory: the kernels need a CUDA device")
+    if c.device != _current_device():
+        raise ValueError(f"the cache is on {c.data.device}, which is not the current device")
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(c.device)
     return getattr(stream, "cuda_stream", stream)

@@ -192,7 +192,7 @@ def test_nan_rows_reach_only_the_queries_that_attend_them(madi):
     """A K or V row that reads back as NaN makes the queries that attend it NaN and no other."""
     import torch
     from madi_b200 import kv4
-    for dt, T in ((torch.float32, 4), (torch.float16, 4), (torch.float16, 80)):
+    for dt, T in ((torch.float32, 4), (torch.float16, 4), (torch.float16, 80), (torch.float16, 140)):
         for which in (0, 1):
             M, H, bad = 150, 2, 100
             c = kv4.Cache.empty(1, H, M)
@@ -276,6 +276,26 @@ def test_captured_calls_on_another_stream(madi, dt, rows, heads, kv_heads, max_t
         call(stream=st)
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, wants[0]))
+
+
+def test_allocations_follow_the_given_stream(madi):
+    """Outputs that a call makes itself are made (and zeroed) on the stream it runs on, given as a
+    stream object or as a handle, the default stream's 0 among them."""
+    import torch
+    from madi_b200 import kv4
+    c, k, v, _ = _rand_store(2, 2, 100, 8)
+    kv4.store(c, k, v)
+    n = torch.tensor([3, 1], dtype=torch.int32, device="cuda")
+    q = torch.randn((2, 4, 128), device="cuda")
+    want = kv4.attn(q, c, 2, n=n), kv4.load(c, 4, n=n, dtype=torch.float32)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for s in (side, side.cuda_stream, torch.cuda.default_stream(), 0):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda._sleep(2_000_000)                    # work that the calls must not wait for or race with
+            got = kv4.attn(q, c, 2, n=n, stream=s), kv4.load(c, 4, n=n, dtype=torch.float32, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][0], want[1][0]) and torch.equal(got[1][1], want[1][1])
 
 
 def test_row_by_row_append_equals_one_store(madi):

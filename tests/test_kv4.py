@@ -81,6 +81,13 @@ def test_attn_refusals():
         _raises(name, kv4.attn, q, c, 6, **{name: i.float()})
 
 
+def test_a_cache_on_another_device_is_refused(monkeypatch):
+    c = _cache()
+    c.device = 1
+    monkeypatch.setattr(kv4, "_current_device", lambda: 0)
+    _raises("not the current device", kv4._raw_stream, None, c)
+
+
 def test_calls_before_init_fail_cleanly():
     from madi_b200 import _lib, build
     build.build()

@@ -14,7 +14,7 @@
 // Both kernels move bytes, and the arithmetic per byte decides how near they come to the memory's
 // rate.  Storing, four lanes share a group (lane j: elements 16 j .. 16 j + 15, code words 2 j and
 // 2 j + 1): with eight lanes of eight elements the range, c and d, which every lane computes for
-// itself, cost as much again.  Loading, eight lanes share a group.  One CTA takes up to 64
+// itself, cost as much again.  Loading, eight lanes share a group.  One CTA takes up to 32
 // consecutive rows of one (slot, head), K and V, so its 32-byte code rows are one run.
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -26,8 +26,8 @@
 namespace madi {
 namespace {
 
-constexpr int kThr = 256;
-constexpr int kRows = 64;      // rows per CTA
+constexpr int kThr = 128;
+constexpr int kRows = 32;      // rows per CTA: small CTAs, whose loads and arithmetic overlap one another's
 constexpr float kLimit = 57344.f;
 
 MADI_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<__half2 *>(&w); }
@@ -203,10 +203,11 @@ MADI_DEV void code_words(const float (&x)[16], float c, float d, uint32_t (&w)[2
     }
 }
 
-// Three CTAs per SM (85 registers): with the 102 it would take, 30.5 us for 8 x 1500 rows of 20 heads
-// f16, with three 26.5; four (64 registers, spilling) 30.8.
+// Bound by its instructions and the latency of its loads: 24.8 us for 8 x 1500 f16 rows of 20 heads (78 MB,
+// 3.2 TB/s).  Six CTAs per SM (80 registers): with the 102 it would take 30.5 us, with 64, spilling, 30.8;
+// with CTAs of 256 threads and 64 rows 26.6.
 template <typename T>
-__global__ void __launch_bounds__(kThr, 3) kv4_store_kernel(uint8_t *__restrict__ data, long long slot_bytes,
+__global__ void __launch_bounds__(kThr, 6) kv4_store_kernel(uint8_t *__restrict__ data, long long slot_bytes,
                                                          long long head_bytes, int max_tok, const T *__restrict__ k,
                                                          const T *__restrict__ v, long long slot_stride,
                                                          long long row_stride, int rows,
@@ -302,6 +303,7 @@ MADI_DEV void st_values(__half *p, const Codes2 &u, __half2 cd, int j) {
     reinterpret_cast<uint4 *>(p)[j] = make_uint4(e[0], e[1], e[2], e[3]);
 }
 
+// Bound by its writes: 24.4 us for those rows as f32 (140 MB, 5.7 TB/s = 88 % of a copy's rate).
 template <typename T>
 __global__ void __launch_bounds__(kThr) kv4_load_kernel(const uint8_t *__restrict__ data, long long slot_bytes,
                                                         long long head_bytes, int max_tok,

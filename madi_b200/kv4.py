@@ -3,8 +3,10 @@
 Thin wrappers of madi_kv4_store / madi_kv4_load / madi_kv4_attn on torch CUDA tensors (format
 and rules: include/madi_q8.h).  36 bytes hold the 64 elements of a (token, kv head), against
 128 in f16 and 256 in f32.  Every call runs on the caller's current torch stream unless a
-stream is given, takes nothing from the host but its arguments' addresses, and can be captured
-in a CUDA graph; positions and lengths are read on the device.
+stream is given; for torch's default stream (handle 0) that is, as in the library's other calls,
+the library stream, which runs in order with it unless madi_set_stream put another in its place.
+A call takes nothing from the host but its arguments' addresses and can be captured in a CUDA
+graph; positions and lengths are read on the device.
 
 A token step's attention takes a few microseconds on the GPU, so the calls are kept short on
 the host: structs are packed in one go, tensors are asked for their properties once.

@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
             put(col, d, ll, oo);
         }
     }
-    if (ns == 1) return;
+    if (W == 1 || ns == 1) return;                          // CTAs of one warp come without a cluster
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     for (int col = rank + tid / kKv4Hd * ns; col < ncol; col += kThr / kKv4Hd * ns) {
         const int d = tid % kKv4Hd;
@@ -592,11 +592,18 @@ cudaError_t launch_stream(const Kv4AttnArgs &a, long long tiles, int ns, cudaStr
 // (8.9 as 1 of 8, 10.3 as 6 of 4), 16 x 20 x 448 ragged 5.7 as 1 of 4 (6.2 as 1 of 8), 8 x 8 x 6000
 // 10.2 as 4 of 8 (10.5 as 8 of 4), 1 x 20 x 1500 4.3 as 6 of 4 (4.7 as 3 of 8), 4 x 8 x 65003 ragged
 // 28.9 as 16 of 8 (32.9 as 8 of 8).
+// With more (slot, kv head, tile)s than that, a CTA's idle warps and its join only take room from the
+// next one: CTAs of two warps, of one for one or two blocks.  Measured with 4, 2 and 1 warps (us):
+// f32, 14 slots x 50 rows x 32 / 4 heads x 52 keys 45.6, 32.4, 28.0; 8 x 48 x 20 x 1500 46.6, 42.4, 71;
+// 8 x 24 x 20 x 128 f16 15.4, 11.4, 15.1; 32 x 5 x 20 x 448 15.1, 10.9, 14.6; x 100 12.7, 9.5, 8.3; one
+// column group: 64 x 1 x 20 x 64 8.5, 6.9, 5.3; 40 x 1 x 20 x 1500 (two sets of warps an SM) 22.3, 25.6, 35.9.
 template <int NT, typename T>
 cudaError_t launch_stream_n(const Kv4AttnArgs &a, long long cols, cudaStream_t st) {
     const long long tiles = (cols + 4 * NT - 1) / (4 * NT), pairs = tiles * a.c.kv_heads * a.c.slots;
     const int nblk = (a.c.max_tok + kKv4Blk - 1) / kKv4Blk;
-    long long room = std::max<long long>((NT == 1 ? 16LL : 8LL) * num_sms() / pairs, 1);
+    long long room = (NT == 1 ? 16LL : 8LL) * num_sms() / pairs;
+    if (room < (NT == 1 ? 2 : 4))
+        return room < 2 && nblk <= 2 ? launch_stream<NT, 1, T>(a, tiles, 1, st) : launch_stream<NT, 2, T>(a, tiles, 1, st);
     if (nblk >= 12 * room) room *= 2;
     const bool cut = nblk <= room;                       // a block per warp
     auto ctas = [&](int w) {

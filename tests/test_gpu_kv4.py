@@ -165,6 +165,18 @@ def test_attn_many_tokens(madi, slots, rows, heads, kv_heads, max_tok, pos, lens
     _attn_case(madi, slots, rows, heads, kv_heads, max_tok, dt, pos=pos, lens=lens, n=n)
 
 
+@pytest.mark.parametrize("dt", [F32, F16])
+@pytest.mark.parametrize("slots,rows,heads,kv_heads,max_tok,mode", [
+    (40, 1, 32, 32, 64, "lens"), (40, 1, 32, 32, 200, "pos"), (20, 5, 32, 32, 100, "pos"), (20, 8, 32, 32, 130, "lens"),
+    (10, 50, 16, 16, 52, "pos"), (10, 20, 32, 32, 128, "lens"), (10, 20, 32, 32, 260, "pos"), (5, 10, 64, 32, 500, "lens")])
+def test_attn_more_heads_than_the_gpu_holds_at_once(madi, slots, rows, heads, kv_heads, max_tok, mode, dt):
+    """Many short caches: smaller CTAs, without a cluster; empty and full ones among them, and padding."""
+    g = np.random.default_rng(17)
+    length = [0, max_tok, max_tok - 1, 1] + [int(x) for x in g.integers(0, max_tok + 1, slots - 4)]
+    n = [int(x) for x in g.integers(0, rows + 1, slots)] if rows > 1 else None
+    _attn_case(madi, slots, rows, heads, kv_heads, max_tok, dt, n=n, **{mode: length})
+
+
 @pytest.mark.parametrize("qscale,spread", [(0.0, 1.0), (1e-6, 1.0), (40.0, 1.0), (1.5, 1e-4), (1.5, 2e4)])
 def test_attn_scales(madi, qscale, spread):
     """Flat and one-hot softmaxes, small and large values: the weights' scale follows d."""

@@ -551,9 +551,11 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
     }
 }
 
-// f16 query columns (rows x query heads per kv head) from which the tensor-core tiles of
-// kv4_flash.cu are faster (8 slots x 20 heads x 1500 keys: 24 columns 40 us here, 42 there; 32: 42, 42;
-// 64: 65, 43; 4 slots x 8 kv heads x 16000 keys: 32 columns 58, 54)
+// f16 query columns (rows x query heads per kv head) from which the tensor-core tiles of kv4_flash.cu
+// are faster: 32, or with a (slot, kv head) per SM what no longer fits one tile here.  Measured (us, here
+// and there): 8 slots x 20 heads x 1500 keys 16 columns 24, 33; 17 42, 34; 32 42, 34; 16 x 20 x 448
+// 20 columns 31, 24.  Fewer pairs: 1 x 20 x 1500 24 columns 11.0, 14.4; 1 x 20 x 448 32 columns 10.9, 11.3;
+// 4 x 8 x 16000 24 columns 59, 50, 4 x 8 x 1000 11.0, 16.3, 2 x 8 x 60000 20 columns 122, 148.
 constexpr int kFlashCols = 32;
 
 template <int NT, int W, typename T>
@@ -595,7 +597,7 @@ cudaError_t launch_stream(const Kv4AttnArgs &a, long long tiles, int ns, cudaStr
 // With more (slot, kv head, tile)s than that, a CTA's idle warps and its join only take room from the
 // next one: CTAs of two warps, of one for one or two blocks.  Measured with 4, 2 and 1 warps (us):
 // f32, 14 slots x 50 rows x 32 / 4 heads x 52 keys 45.6, 32.4, 28.0; 8 x 48 x 20 x 1500 46.6, 42.4, 71;
-// 8 x 24 x 20 x 128 f16 15.4, 11.4, 15.1; 32 x 5 x 20 x 448 15.1, 10.9, 14.6; x 100 12.7, 9.5, 8.3; one
+// 32 x 5 x 20 x 448 15.1, 10.9, 14.6; x 100 12.7, 9.5, 8.3; one
 // column group: 64 x 1 x 20 x 64 8.5, 6.9, 5.3; 40 x 1 x 20 x 1500 (two sets of warps an SM) 22.3, 25.6, 35.9.
 template <int NT, typename T>
 cudaError_t launch_stream_n(const Kv4AttnArgs &a, long long cols, cudaStream_t st) {
@@ -634,7 +636,8 @@ cudaError_t launch_stream_t(const Kv4AttnArgs &a, long long cols, cudaStream_t s
 
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, bool f16, cudaStream_t st) {
     const long long cols = (long long)a.rows * (a.heads / a.c.kv_heads);
-    if (f16 && cols >= kFlashCols) return launch_kv4_flash(a, st);
+    if (f16 && (cols >= kFlashCols || (cols > 16 && (long long)a.c.slots * a.c.kv_heads >= num_sms())))
+        return launch_kv4_flash(a, st);
     return f16 ? launch_stream_t<__half>(a, cols, st) : launch_stream_t<float>(a, cols, st);
 }
 

@@ -168,7 +168,8 @@ def test_attn_many_tokens(madi, slots, rows, heads, kv_heads, max_tok, pos, lens
 @pytest.mark.parametrize("dt", [F32, F16])
 @pytest.mark.parametrize("slots,rows,heads,kv_heads,max_tok,mode", [
     (40, 1, 32, 32, 64, "lens"), (40, 1, 32, 32, 200, "pos"), (20, 5, 32, 32, 100, "pos"), (20, 8, 32, 32, 130, "lens"),
-    (10, 50, 16, 16, 52, "pos"), (10, 20, 32, 32, 128, "lens"), (10, 20, 32, 32, 260, "pos"), (5, 10, 64, 32, 500, "lens")])
+    (10, 50, 16, 16, 52, "pos"), (10, 20, 32, 32, 128, "lens"), (10, 20, 32, 32, 260, "pos"), (5, 10, 64, 32, 500, "lens"),
+    (10, 17, 16, 16, 97, "pos"), (5, 9, 64, 32, 300, "lens")])
 def test_attn_more_heads_than_the_gpu_holds_at_once(madi, slots, rows, heads, kv_heads, max_tok, mode, dt):
     """Many short caches: smaller CTAs, without a cluster; empty and full ones among them, and padding."""
     g = np.random.default_rng(17)

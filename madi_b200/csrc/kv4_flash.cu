@@ -4,8 +4,9 @@
 // Same mathematics as the streaming form (kv4_attn.cu), as matrix products of 128 x 96 tiles:
 //     S = Q K^T,  K = c + d n':   Q (d n')^T + sum(Q) c^T
 //     O = P V,    V = c + d n':   P (d n')   + sum_j P_j c_j
-// d has 8 significant bits and |n'| <= 8, so d n' is exact in f16 and only P is rounded (2^-11 at
-// most, as the output itself is): the keys' c enters S as a fifth K = 16 step with sum(Q) as two
+// d has 8 significant bits and |n'| <= 8, so d n' is exact in f16 and only P is rounded (by 2^-11 of
+// itself, as the output is, and by 2^-38 of the row's largest where it is below 2^-27 of that; the
+// streaming form keeps 22 bits of it): the keys' c enters S as a fifth K = 16 step with sum(Q) as two
 // f16 parts, the values' c as one more column of V, beside a column of ones that gives the sum of
 // the weights.  Rounding c + d n' to f16 instead would add two more errors of the output's own size.
 //
@@ -54,7 +55,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kIdescS = idesc_f16_f32(kQT, kKT);
 constexpr uint32_t kIdescPV = idesc_f16_f32(kQT, kKv4Hd + 16) | (1u << 16);      // V: N-contiguous
 constexpr int kMaxNs = 8;
-constexpr float kSlack = 8.f;                  // base-2 head room of the softmax reference
+// A weight is 2^kPOff times 2^(score - reference); the reference lies at most 2^kSlack below the largest score so
+// far, so the largest weight is between 2^13 and 2^15 and f16 holds weights down to 2^-27 of it with all its bits
+// (those behind a dominant key count as much as any when that key's value is small; with the largest at 1
+// to 2^8, half of a result was lost at 2^-22).  Slack 2 for 8 costs about 1 %: 2 x 1024 rows x 32 heads,
+// 16640 keys 351.8 us, 348.4 with 8, 349.6 with 4, 356.0 with 0.
+constexpr float kSlack = 2.f, kPOff = 13.f;
 constexpr int kPartW = kKv4Hd + 2;             // a row's partial: O, m, l
 
 template <int kX, int kNS> struct __align__(16) FlashShared {
@@ -396,11 +402,12 @@ __global__ void __launch_bounds__(FlashCfg<kX>::kThr, FlashCfg<kX>::kPerSm)
                     for (int i = 0; i < 32; i += 2)
                         mx[(i >> 1) & 7] = max3f(mx[(i >> 1) & 7], score(c, i), score(c, i + 1));
                 const float mxr = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-                // The reference moves only when a maximum passes it by more than 2^kSlack: weights up
-                // to 2^kSlack are as good in f16 and f32, and O is rescaled in few tiles instead of most.
+                // The reference moves only when a maximum passes it by more than 2^kSlack, so O is rescaled in
+                // few tiles instead of most.
                 const float mt = mxr * scale;
                 mn = mt > m + kSlack ? mt : m;
                 const float ml = mn == -CUDART_INF_F ? 0.f : mn;          // no key yet
+                const float off = kPOff - ml;
                 alpha = mn == m ? 1.f : ex2_approx(m - ml);               // exactly 1 when it did not move
                 if (j > 0) {
                     if (!warp_wait_all(&sh->o_done[x], (uint32_t)(j - 1) & 1u, abort_flag, a.dev_err)) return false;
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(FlashCfg<kX>::kThr, FlashCfg<kX>::kPerSm)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         float a0, a1;
-                        fma2(a0, a1, score(c, i), score(c, i + 1), scale, scale, -ml, -ml);
+                        fma2(a0, a1, score(c, i), score(c, i + 1), scale, scale, off, off);
                         pp[i >> 1] = h2_as_u32(__floats2half2_rn(ex2_approx(a0), ex2_approx(a1)));
                     }
                     tmem_st16(tb + kPCol + 16 * c, pp);

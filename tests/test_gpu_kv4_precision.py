@@ -1,0 +1,81 @@
+"""How near attention over the 4-bit K/V cache comes to the exact result on inputs that are hard for
+it: one key that outweighs all others by many orders while its value is small, values of very
+different size.  The exact result is computed in 64 bits from the rows read back (which
+test_gpu_kv4.py compares bit for bit)."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -23             # a tensor-core sum may cut its last place instead of rounding it
+LOG2E = math.log2(math.e)
+
+
+def _gen(seed):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return lambda *s: torch.randn(s, generator=g, device="cuda")
+
+
+def _stored(K, V, kv_heads):
+    """(cache, k, v [S][H][M][64] f64 as read back, |c| + 16 d of each [S][H][M] f64)."""
+    import torch
+    from madi_b200 import kv4
+    S, M, _ = K.shape
+    c = kv4.Cache.empty(S, kv_heads, M)
+    kv4.store(c, K, V)
+    k, v = (x.double().view(S, M, kv_heads, 64).transpose(1, 2) for x in kv4.load(c, M, dtype=torch.float32))
+    mags = []
+    for at in (2048, 2048 + 2304):
+        cd = c.data[..., at:at + 256].contiguous().view(torch.float16).double().reshape(S, kv_heads, -1, 2)[:, :, :M]
+        mags.append(cd[..., 0].abs() + 16 * cd[..., 1])
+    return c, k, v, mags
+
+
+def _split(q, kv_heads):
+    """q [S][T][heads * 64] -> [S][kv_heads][T * group][64] f64."""
+    S, T, W = q.shape
+    return q.double().view(S, T, kv_heads, -1, 64).permute(0, 2, 1, 3, 4).reshape(S, kv_heads, -1, 64)
+
+
+def _sink(seed, rows, heads, kv_heads, M, gap, noise, value=0.0):
+    """Every query row prefers key 0 to the others by about `gap` nats; its value is `value` times theirs."""
+    rn = _gen(seed)
+    one = rn(1, 1, kv_heads, 1, 64)
+    q = one.expand(1, rows, kv_heads, heads // kv_heads, 64).reshape(1, rows, heads * 64).contiguous()
+    K = noise * rn(1, M, kv_heads, 64)
+    x = one[:, 0, :, 0]
+    K[:, 0] = gap * 8 * x / (x * x).sum(-1, keepdim=True)
+    V = rn(1, M, kv_heads, 64) + 1.0
+    V[:, 0] *= value
+    return q, K.reshape(1, M, -1), V.reshape(1, M, -1)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(40, 1, 1), (100, 4, 2)])
+@pytest.mark.parametrize("M", [448, 1500, 20000])
+@pytest.mark.parametrize("gap,noise", [(8, 0.5), (12, 0.0), (15, 0.0), (15, 0.5), (17, 0.0), (17, 0.5)])
+def test_f16_weights_behind_a_dominant_key(madi, rows, heads, kv_heads, M, gap, noise):
+    """Many f16 rows: a weight is rounded to f16 by at most 2^-11 of itself, and by 2^-38 of the largest
+    where it is smaller than 2^-27 of that.  Beside it, as in kv4_ref.attend: the scores' sums (16 u of
+    the sum of magnitudes), the subtraction in base 2, exp2, the products' sums (2 M / 16 + 16 steps), and the
+    output's rounding."""
+    import torch
+    from madi_b200 import kv4
+    q, K, V = _sink(rows + M + gap, rows, heads, kv_heads, M, gap, noise)
+    q = q.half()
+    c, k, v, (kmag, vmag) = _stored(K, V, kv_heads)
+    got = kv4.attn(q, c, heads).double()
+    x = _split(q, kv_heads)
+    z = x @ k.transpose(-1, -2) / 8
+    z = z - z.amax(-1, keepdim=True)
+    p = torch.softmax(z, -1)
+    mag = x.abs().sum(-1, keepdim=True) / 8 * (1.5 * kmag).unsqueeze(2)           # |q| (|c| + 24 d) / 8
+    ep = (16 * U * mag + U * LOG2E * z.abs() + 4 * U).amax(-1, keepdim=True)
+    want, a, b = p @ v, p @ v.abs(), p @ vmag.unsqueeze(-1)
+    tol = 2 * ep * a + (2 * M / 16 + 16) * U * b + 2 * 2.0 ** -11 * a + 2 * M * 2.0 ** -38 * v.abs().max()
+    tol = tol + torch.clamp(2.0 ** -11 * (want.abs() + tol), min=2.0 ** -25)
+    err = (_split(got, kv_heads) - want).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), f"error {err.max().item():.3e}, {(err / tol).max().item():.2f} x its bound"

@@ -21,10 +21,14 @@
 //     of a byte) or z 2^-20 (high nibble): one logic instruction unpacks two codes, and the
 //     power of two goes into q (keys) or into the result (values);
 //   * the eight columns of an instruction hold four query columns as two f16 numbers each,
-//     x = hi + lo with hi on a fixed grid: hi's products and their sums are exact in the tensor
-//     core, and lo's are 2^10 times smaller, so f32 queries and outputs lose nothing to
-//     f16 operands or to how the tensor core aligns its addends (with hi = f16(x), whose
-//     products differ in exponent, f32 results were 2e-5 off in norm);
+//     x = hi + lo.  The tensor core aligns a subnormal as if it were a normal number, and cuts
+//     there: with hi = f16(x), whose products differ in exponent, f32 results were 2e-5 off in
+//     norm.  So queries (and the weights of f16 outputs) have hi on a fixed grid, where its
+//     products and their sums are exact, and lo's are 2^10 times smaller.  A query's elements may
+//     share a grid: their products add up to one score.  The weights of f32 outputs may not: keys
+//     behind a dominant one whose value is small make up the result with weights of any size (on a
+//     grid it was up to 7e-5 off in norm).  There hi is f16(x), and the values' codes become normal
+//     numbers n' by one more instruction a pair (8 slots x 20 heads x 1500 keys 8.2 -> 8.8 us);
 //   * S is computed as [keys x columns], O as [dims x columns]; the weights turn from
 //     the first product's result into the second's operand by one movmatrix a key group.
 //   * ldmatrix brings the codes, as 16-bit elements, straight into the operands' places; its
@@ -96,22 +100,37 @@ MADI_DEV uint32_t cluster_id_x() {
 constexpr float kGrid8 = 12582912.f * 8.f, kGrid4 = 12582912.f * 4.f;
 // Exponent that the largest d of the keys so far is brought to in the weights' scale.
 template <typename T> constexpr int kTop = sizeof(T) == 4 ? 14 : 12;
-// Two weights x < 2^(kTop + 1) as {hi, lo} f16 pairs, hi a multiple of 4.  f32 outputs: hi is
-// the nearest f16, on the grid of 4 where f16 is finer, so that lo is at most 2^-12 of x (or 2 of
-// 2^15).  f16 outputs: below 2^13 every multiple of 4 is an f16, and lo, at most 2, leaves 2^-24
-// of the largest weight off.
+// Two weights x < 2^(kTop + 1) as {hi, lo} f16 pairs.  f32 outputs: hi is the nearest f16 and lo the rest
+// times 2^11, so that x keeps 22 bits down to 2^-28 of the largest weight (lo as it is, on the grid of
+// the f16 form, left weights below 2^-12 of it 11 bits, and some of their results 2^-14 off).  f16
+// outputs: hi is a multiple of 4, which below 2^13 is an f16, and lo, at most 2, leaves 2^-24 of
+// the largest weight or 2^-12 of x off.
+constexpr float kLoUp = 2048.f;
 template <typename T>
 MADI_DEV void split_weights(float x0, float x1, uint32_t &w0, uint32_t &w1) {
-    float h0 = x0, h1 = x1, l0, l1;
-    if (sizeof(T) == 4) {
-        h0 = __half2float(__float2half_rn(x0));
-        h1 = __half2float(__float2half_rn(x1));
+    float l0, l1;
+    if constexpr (sizeof(T) == 4) {
+        const __half2 h = __floats2half2_rn(x0, x1);
+        const float2 hf = __half22float2(h);
+        mul2(l0, l1, x0, x1, kLoUp, kLoUp);
+        fma2(l0, l1, hf.x, hf.y, -kLoUp, -kLoUp, l0, l1);
+        const uint32_t hi = h2_as_u32(h), lo = h2_as_u32(__floats2half2_rn(l0, l1));
+        w0 = __byte_perm(hi, lo, 0x5410);
+        w1 = __byte_perm(hi, lo, 0x7632);
+    } else {
+        float h0, h1;
+        add2(h0, h1, x0, x1, kGrid4, kGrid4);
+        add2(h0, h1, h0, h1, -kGrid4, -kGrid4);
+        fma2(l0, l1, h0, h1, -1.f, -1.f, x0, x1);
+        w0 = h2_as_u32(__floats2half2_rn(h0, l0));
+        w1 = h2_as_u32(__floats2half2_rn(h1, l1));
     }
-    add2(h0, h1, h0, h1, kGrid4, kGrid4);
-    add2(h0, h1, h0, h1, -kGrid4, -kGrid4);
-    fma2(l0, l1, h0, h1, -1.f, -1.f, x0, x1);
-    w0 = h2_as_u32(__floats2half2_rn(h0, l0));
-    w1 = h2_as_u32(__floats2half2_rn(h1, l1));
+}
+// Two codes of a word under the mask of tile i as f16 numbers: n' of the low nibbles (even i), 16 n' of
+// the high ones.
+MADI_DEV uint32_t codes_f16(uint32_t w, int i) {
+    const uint32_t v = (w & ((i & 1) ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;     // 1024 + z, 1024 + 16 z
+    return h2_as_u32(__hsub2(*reinterpret_cast<const __half2 *>(&v), __float2half2_rn((i & 1) ? 1152.f : 1032.f)));
 }
 // Elements p[0 .. 7] and p[32 .. 39].
 MADI_DEV void ld16(const float *p, float (&f)[16]) {
@@ -264,13 +283,20 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
         for (int i = 0; i < 8; ++i) tot[nt][i] = 0.f;
     }
     // o: sums of z w (w the weights' parts), o8: of 8 w, in every row; z - 8 = n'.  The accumulators'
-    // columns 2t, 2t + 1 are this lane's column t; odd tiles are in units of 2^-20.
+    // columns 2t, 2t + 1 are this lane's column t; odd tiles are in units of 2^-20.  f32: sums of n' w,
+    // odd tiles of 16 n' w.
     auto flush = [&](int nt, float f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float e = (i & 1) ? -16.f : -1.f;
-            const float x = fmaf(e, o8[nt][0], o[nt][i][0]) + fmaf(e, o8[nt][1], o[nt][i][1]);
-            const float y = fmaf(e, o8[nt][0], o[nt][i][2]) + fmaf(e, o8[nt][1], o[nt][i][3]);
+            float x, y;
+            if constexpr (kF32) {
+                x = fmaf(o[nt][i][1], 1.f / kLoUp, o[nt][i][0]);
+                y = fmaf(o[nt][i][3], 1.f / kLoUp, o[nt][i][2]);
+            } else {
+                x = fmaf(e, o8[nt][0], o[nt][i][0]) + fmaf(e, o8[nt][1], o[nt][i][1]);
+                y = fmaf(e, o8[nt][0], o[nt][i][2]) + fmaf(e, o8[nt][1], o[nt][i][3]);
+            }
             tot[nt][2 * i] = (tot[nt][2 * i] + x) * f;
             tot[nt][2 * i + 1] = (tot[nt][2 * i + 1] + y) * f;
             o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
@@ -278,10 +304,12 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
         o8[nt][0] = o8[nt][1] = o8[nt][2] = o8[nt][3] = 0.f;
     };
     // The weights p d enter the second product times 2^we, with d's largest exponent so far
-    // brought to kTop.  hi is a multiple of 4, so sums of z hi are exact up to 2^26 = 15 x 2^15 x 136
-    // keys (f16 outputs: x 2^13 x 546).  After kFlush blocks of 64 keys, and when the scale moves,
-    // the products' sums are added to f32 totals and start anew: a total that had been scaled by
-    // something else than its grid would be cut to the grid by the next product.
+    // brought to kTop.  f16 outputs: the codes are the subnormals z 2^-24, whose products the tensor core
+    // aligns as if they were 2^10 larger and cuts there; hi is a multiple of 4 so that the sums of z hi are
+    // exact all the same, up to 2^26 = 15 x 2^13 x 546 keys.  f32 outputs: hi has all its bits, so the codes
+    // come as the normal numbers n', whose sums lose no more than f32 ones.  After kFlush blocks of 64
+    // keys, and when the scale moves, the products' sums are added to f32 totals and start anew: a total that
+    // had been scaled by something else than its grid would be cut to the grid by the next product.
     constexpr int kFlush = kF32 ? 2 : 4;
     float dcap = 0.f, wscale = 1.f;                         // largest d the scale allows for; 2^we
     int we = 0, since = 0;                                  // since: blocks since the sums were flushed
@@ -435,9 +463,13 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t mask = (i & 1) ? 0x00F000F0u : 0x000F000Fu;
                     const uint32_t u = vw[i & 2], w = vw[(i & 2) + 1];
-                    mma16816(o[nt][i], u & mask, (u >> 8) & mask, w & mask, (w >> 8) & mask, b0, b1);
+                    if constexpr (kF32)
+                        mma16816(o[nt][i], codes_f16(u, i), codes_f16(u >> 8, i), codes_f16(w, i), codes_f16(w >> 8, i), b0,
+                                 b1);
+                    else
+                        mma16816(o[nt][i], u & mask, (u >> 8) & mask, w & mask, (w >> 8) & mask, b0, b1);
                 }
-                mma16816(o8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
+                if constexpr (!kF32) mma16816(o8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
             }
         }
         __syncwarp();                                       // the stage's last reads, before it is filled again
@@ -469,7 +501,7 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
             wp[lane * kPart + 1] = 0.f;
         }
     } else {
-        const float back = pow2i(-we) * kUp24;
+        const float back = pow2i(-we) * (kF32 ? 1.f : kUp24);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float ls = l[nt][0] + l[nt][1], os = oc[nt][0] + oc[nt][1];

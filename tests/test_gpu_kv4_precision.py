@@ -79,3 +79,57 @@ def test_f16_weights_behind_a_dominant_key(madi, rows, heads, kv_heads, M, gap, 
     err = (_split(got, kv_heads) - want).abs()
     assert torch.isfinite(got).all()
     assert (err <= tol).all(), f"error {err.max().item():.3e}, {(err / tol).max().item():.2f} x its bound"
+
+
+def _norm_error(q, c, k, v, heads, kv_heads):
+    import torch
+    from madi_b200 import kv4
+    got = _split(kv4.attn(q, c, heads), kv_heads)
+    want = torch.softmax(_split(q, kv_heads) @ k.transpose(-1, -2) / 8, -1) @ v
+    assert torch.isfinite(got).all()
+    return ((got - want).norm() / want.norm()).item()
+
+
+# f32 results in norm: 1e-6 for the sums (a plain f32 form is 2e-7 to 5e-7 off, see test_gpu_kv4.py)
+F32_SUMS = 1e-6
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 1, 1), (1, 12, 3), (6, 1, 1), (20, 2, 1)])
+@pytest.mark.parametrize("M", [448, 1500, 20000])
+@pytest.mark.parametrize("gap", [0.0, 8.3, 10.0, 13.0, 20.0])
+def test_f32_weights_behind_a_dominant_key(madi, rows, heads, kv_heads, M, gap):
+    """All keys but the first score 0 and hold the same values, so that a rounding of their weight is not
+    averaged out.  The first scores `gap` nats: q's scaling to base 2, the score's three operations and the
+    subtraction round at 2^-24 of it each, and the weights behind it carry that."""
+    import torch
+    rn = _gen(M + rows)
+    q = torch.zeros((2, rows, heads * 64), device="cuda")
+    q[..., ::64] = 8.0
+    K = torch.zeros((2, M, kv_heads, 64), device="cuda")
+    K[:, 0, :, 0] = gap
+    V = torch.where(rn(1, 1, kv_heads, 64) > 0, 1.0, -1.0) * (0.7 + 0.3 * rn(1, 1, kv_heads, 64).abs())
+    V = V.repeat(2, M, 1, 1)
+    V[:, 0] = 0.0
+    c, k, v, _ = _stored(K.reshape(2, M, -1), V.reshape(2, M, -1), kv_heads)
+    err = _norm_error(q, c, k, v, heads, kv_heads)
+    assert err <= F32_SUMS + 5 * 2.0 ** -24 * gap, f"{err:.2e}"
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 1, 1), (6, 1, 1), (20, 2, 1)])
+@pytest.mark.parametrize("M", [300, 1000, 20000])
+@pytest.mark.parametrize("ratio", [10.0, 1e3, 1e4])
+def test_f32_values_beside_a_large_one_of_no_weight(madi, rows, heads, kv_heads, M, ratio):
+    """One key some 60 nats below the others holds values `ratio` times as large.  The others' scores, within
+    6 nats of one another, differ, so that their weights need all bits; they round as above."""
+    import torch
+    rn = _gen(M + rows)
+    one = rn(1, 1, kv_heads, 1, 64)
+    q = one.expand(1, rows, kv_heads, heads // kv_heads, 64).reshape(1, rows, heads * 64).contiguous()
+    K = rn(1, M, kv_heads, 64)
+    x = one[:, 0, :, 0]
+    K[:, 3] = -60 * 8 * x / (x * x).sum(-1, keepdim=True)
+    V = rn(1, M, kv_heads, 64)
+    V[:, 3] *= ratio
+    c, k, v, _ = _stored(K.reshape(1, M, -1), V.reshape(1, M, -1), kv_heads)
+    err = _norm_error(q, c, k, v, heads, kv_heads)
+    assert err <= F32_SUMS + 5 * 2.0 ** -24 * 6, f"{err:.2e}"

@@ -114,14 +114,14 @@ template <> struct Src16<__half> {
 // The step d: the least number with 8 significant bits that is a multiple of 2^-24, with
 // 8 d >= c - lo and 7 d >= hi - c.  (Differences rounded up compare with 7 d and 8 d as the exact
 // ones do, since both products are f32 numbers.)  An estimate from below by the reciprocal of 7 is
-// raised to the grid, and raised once more if 7 d falls short.
+// raised to the grid, and raised once more if 7 d falls short, or 8 d: an eighth of a few 2^-149 is 0.
 MADI_DEV float step_of(float lo, float hi, float c) {
-    const float up = __fsub_ru(hi, c);
-    const float r = fmaxf(__fsub_ru(c, lo) * 0.125f, up * 0.14285707f);       // (1/7)(1 - 5e-7)
+    const float up = __fsub_ru(hi, c), down = __fsub_ru(c, lo);
+    const float r = fmaxf(down * 0.125f, up * 0.14285707f);       // (1/7)(1 - 5e-7)
     float d;
     if (r < 7.62939453125e-06f) {                        // below 2^-17 the multiples of 2^-24 are the coarser grid
         d = ceilf(r * 16777216.f) * 5.9604644775390625e-08f;
-        if (d * 7.f < up) d += 5.9604644775390625e-08f;
+        if (d * 7.f < up || d * 8.f < down) d += 5.9604644775390625e-08f;
     } else {
         uint32_t b = (__float_as_uint(r) + 0xFFFFu) & 0xFFFF0000u;
         if (__uint_as_float(b) * 7.f < up) b += 0x10000u;

@@ -1,10 +1,13 @@
 """How near attention over the 4-bit K/V cache comes to the exact result on inputs that are hard for
 it: one key that outweighs all others by many orders while its value is small, values of very
 different size.  The exact result is computed in 64 bits from the rows read back (which
-test_gpu_kv4.py compares bit for bit)."""
+test_gpu_kv4.py compares bit for bit).  And the smallest numbers a row to store can hold."""
 import math
 
+import numpy as np
 import pytest
+
+from tests import kv4_ref as R
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +136,27 @@ def test_f32_values_beside_a_large_one_of_no_weight(madi, rows, heads, kv_heads,
     c, k, v, _ = _stored(K.reshape(1, M, -1), V.reshape(1, M, -1), kv_heads)
     err = _norm_error(q, c, k, v, heads, kv_heads)
     assert err <= F32_SUMS + 5 * 2.0 ** -24 * 6, f"{err:.2e}"
+
+
+def test_store_of_the_smallest_numbers(madi):
+    """Groups of a few 2^-149 on one side or both, whose step has to be 2^-24 and not 0: the same bytes
+    as the format's definition gives."""
+    import torch
+    from madi_b200 import kv4
+    tiny = np.float32(2.0 ** -149)
+    rows = [np.full(64, a) for a in range(-12, 13)]
+    for lo in range(-9, 10):
+        for hi in range(lo + 1, 10):
+            rows.append(np.where(np.arange(64) % 3 == 0, lo, hi))
+    g = np.random.default_rng(2)
+    rows += [np.rint(g.uniform(-1, 1, 64) * 2.0 ** b) for b in (4, 10, 20, 30, 60, 120, 122, 124, 125, 126, 127)]
+    x = (np.array(rows, dtype=np.float64) * float(tiny)).astype(np.float32)
+    c = kv4.Cache.empty(1, 1, len(x))
+    X = torch.from_numpy(x[None]).cuda()
+    kv4.store(c, X, X)
+    z, cc, dd = R.quantise(x)
+    assert (dd[np.abs(x).max(-1) > 0] >= 2.0 ** -24).all()
+    torch.cuda.synchronize()
+    for kv in (0, 1):
+        gz, gc, gd = R.unpack(c.data.cpu().numpy(), kv, len(x))
+        assert np.array_equal(gc[0, 0], cc) and np.array_equal(gd[0, 0], dd) and np.array_equal(gz[0, 0], z)

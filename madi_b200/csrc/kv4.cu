@@ -206,13 +206,13 @@ MADI_DEV void code_words(const float (&x)[16], float c, float d, uint32_t (&w)[2
 // Bound by its instructions and the latency of its loads: 24.8 us for 8 x 1500 f16 rows of 20 heads (78 MB,
 // 3.2 TB/s).  Six CTAs per SM (80 registers): with the 102 it would take 30.5 us, with 64, spilling, 30.8;
 // with CTAs of 256 threads and 64 rows 26.6.
+// No pointer of these kernels is __restrict__: their memory is written while they are already resident (by the
+// kernel before them, until pdl_wait), so loads through the read-only path would be wrong.
 template <typename T>
-__global__ void __launch_bounds__(kThr, 6) kv4_store_kernel(uint8_t *__restrict__ data, long long slot_bytes,
-                                                         long long head_bytes, int max_tok, const T *__restrict__ k,
-                                                         const T *__restrict__ v, long long slot_stride,
-                                                         long long row_stride, int rows,
-                                                         const uint32_t *__restrict__ pos,
-                                                         const uint32_t *__restrict__ n) {
+__global__ void __launch_bounds__(kThr, 6) kv4_store_kernel(uint8_t *data, long long slot_bytes, long long head_bytes,
+                                                            int max_tok, const T *k, const T *v, long long slot_stride,
+                                                            long long row_stride, int rows, const uint32_t *pos,
+                                                            const uint32_t *n) {
     pdl_trigger();
     pdl_wait();
     const int h = blockIdx.y, r0 = (int)blockIdx.x * kRows, s = blockIdx.z;
@@ -305,12 +305,10 @@ MADI_DEV void st_values(__half *p, const Codes2 &u, __half2 cd, int j) {
 
 // Bound by its writes: 24.4 us for those rows as f32 (140 MB, 5.7 TB/s = 88 % of a copy's rate).
 template <typename T>
-__global__ void __launch_bounds__(kThr) kv4_load_kernel(const uint8_t *__restrict__ data, long long slot_bytes,
-                                                        long long head_bytes, int max_tok,
-                                                        T *__restrict__ k, T *__restrict__ v, long long slot_stride,
-                                                        long long row_stride, int rows,
-                                                        const uint32_t *__restrict__ pos,
-                                                        const uint32_t *__restrict__ n) {
+__global__ void __launch_bounds__(kThr) kv4_load_kernel(const uint8_t *data, long long slot_bytes, long long head_bytes,
+                                                        int max_tok, T *k, T *v, long long slot_stride,
+                                                        long long row_stride, int rows, const uint32_t *pos,
+                                                        const uint32_t *n) {
     constexpr int kB = 2;                                     // rows whose loads are in flight together
     pdl_trigger();
     pdl_wait();

@@ -372,7 +372,9 @@ typedef struct madi_kv4 {
 size_t madi_kv4_bytes(int slots, int kv_heads, int max_tok);
 
 /* K and V rows beside the cache: element (s, i, j) of k and of v at s * slot_stride +
- * i * row_stride + j, i < rows, j < kv_heads * 64; 16-byte aligned rows; dtype MADI_F32 or MADI_F16.
+ * i * row_stride + j, i < rows (at most 2^20), j < kv_heads * 64; 16-byte aligned rows that do not
+ * overlap, slot by slot or row by row (all slots' rows i before their rows i + 1); dtype MADI_F32 or
+ * MADI_F16.
  * Row i of slot s belongs to cache row pos[s] + i, for i < n[s].  pos, n: u32 [slots] on the device
  * (read there, so a graph can replay them); NULL: 0 and `rows`. */
 typedef struct madi_kv4_rows {

@@ -1115,15 +1115,19 @@ int kv4_check(const char *who, const madi_kv4 *c, int dtype, int rows) {
         return fail(MADI_EINVAL, "%s: the current device is not device %d, which madi_init bound", who, S.device);
     return MADI_OK;
 }
-// Row tensors: non-null, 16-byte aligned rows that do not overlap one another.
+// Row tensors: non-null, 16-byte aligned rows that do not overlap one another; slot-major, or row-major (a
+// token's rows of all slots side by side).
 int kv4_rows_check(const char *who, const char *what, const void *p, int dtype, int slots, int rows, int64_t slot,
                    int64_t row, int64_t width) {
     const int64_t unit = dtype == MADI_F32 ? 4 : 8;
     if (!p) return fail(MADI_EINVAL, "%s: null %s", who, what);
     if (!aligned(p, 16) || slot % unit || row % unit)
         return fail(MADI_EINVAL, "%s: rows of %s must be 16-byte aligned", who, what);
-    if ((rows > 1 && (row < width || row > kKv4MaxStride)) ||
-        (slots > 1 && (slot < (rows > 1 ? (rows - 1) * row : 0) + width || slot > kKv4MaxStride)))
+    if (rows == 1) row = 0;                                  // a stride that no element takes
+    if (slots == 1) slot = 0;
+    const bool in_range = row >= 0 && row <= kKv4MaxStride && slot >= 0 && slot <= kKv4MaxStride;
+    if (!in_range || (rows > 1 && row < width) || (slots > 1 && slot < width) ||
+        (rows > 1 && slots > 1 && slot < (rows - 1) * row + width && row < (slots - 1) * slot + width))
         return fail(MADI_EINVAL, "%s: strides %lld / %lld of %s (rows of %lld)", who, (long long)slot, (long long)row, what,
                     (long long)width);
     return MADI_OK;

@@ -25,7 +25,7 @@ BLOCK_TOKENS = 64          # tokens per block
 BLOCK_BYTES = 4608         # K and V of a block: codes and (c, d) of each
 _DT = {torch.float32: MADI_F32, torch.float16: MADI_F16}
 _U32 = (torch.int32, torch.uint32)
-_current_device = torch._C._cuda_getDevice
+_current_device = getattr(torch._C, "_cuda_getDevice", None)       # absent in torch without CUDA
 # the structs of include/madi_q8.h
 _CACHE = struct.Struct("=Qiii4x").pack
 _ROWS = struct.Struct("=QQQQqqii").pack

@@ -577,9 +577,11 @@ cudaError_t launch_flash(const Kv4AttnArgs &a, cudaStream_t st) {
     const long long hb = (long long)nblk * kKv4Block, ctas = tiles * a.c.kv_heads * a.c.slots;
     const long long room = (long long)num_sms() * Cfg::kPerSm;
     // Cluster size.  A CTA costs about 7 us beside its key tiles of 1.7 us each (4 tiles' time),
-    // one of a cluster 16 us (9 tiles'); take the size with the least rounds x time.  Long shares are
-    // cut once more where causal or ragged lengths would leave few rounds unbalanced (2 x 1024 rows x
-    // 32 heads, 16640 keys: 377 us at 1, 349 at 2, 404 at 3).
+    // one of a cluster 16 us (9 tiles'); take the size with the least rounds x time.  Two or three rounds of
+    // long shares are cut once more where slots may differ in length, which would leave the rounds unbalanced: 2 x
+    // 1024 rows x 32 / 8 heads, 16640 keys, at 1 and 2 CTAs: ragged pos 379, 351 us, ragged lens 390, 359; equal pos
+    // 506, 547.  Whole caches (515, 558) and what fits one round are not: 2 x 128 rows x 32 / 8 heads x 60000 at 4
+    // and 8: 243, 400, ragged lens 244, 266; 1 x 2000 x 8 / 2 x 30000 at 2 and 4: 240, 252.
     const long long ktiles = (a.c.max_tok + kKT - 1) / kKT;
     int ns = 1;
     long long best = 0;
@@ -591,7 +593,8 @@ cudaError_t launch_flash(const Kv4AttnArgs &a, cudaStream_t st) {
             ns = c;
         }
     }
-    while (ns * 2 <= kMaxNs && ctas * ns < 4 * room && ktiles / (ns * 2) >= 64) ns *= 2;
+    const bool unequal = a.c.slots > 1 && (a.pos || a.lens || a.n);
+    while (unequal && ns * 2 <= kMaxNs && ctas * ns > room && ctas * ns < 4 * room && ktiles / (ns * 2) >= 64) ns *= 2;
     if (tiles * a.c.kv_heads * ns > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_k(kv4_flash_kernel<kX>, dim3((unsigned)(tiles * a.c.kv_heads * ns), (unsigned)a.c.slots), Cfg::kThr,
                     Cfg::kSmem, st, ns, a, hb * a.c.kv_heads, hb, group, (int)tiles, ns);

@@ -151,9 +151,10 @@ MADI_DEV float code_exact(float x, float c, float d, float inv) {
 // ((n'3 16 + n'2) 16 + n'1) 16 + n'0, exactly.  The quotient is taken of t + 2^-18 d, t = x - c, so
 // that a half, which f16 inputs hit once in some hundred elements, is rounded up although the
 // reciprocal is not exact (its error and the product's are 2^-19 together).  The remainder r = t -
-// n' d is exact and has to lie in [-d/2, d/2): codes that it shows to be wrong, within 2^-18 of a
-// border, are rare, and then all sixteen are decided one by one.  r = -d/2 is right if t is x - c
-// itself or below it: that is looked at only where it occurs.
+// n' d has to lie in [-d/2, d/2): codes that it shows to be wrong, within 2^-18 of a border, are rare, and
+// then all sixteen are decided one by one.  Where r = -d/2, two things are looked at: r is exact but for
+// a t just below d/2 = 2^k (its last place is half of r's), so t - (n' - 1/2) d, which is, decides; and if that is
+// 0, x - c must not lie below t.
 MADI_DEV void code_words(const float (&x)[16], float c, float d, uint32_t (&w)[2]) {
     constexpr float kMagic = 12582912.f;
     const float inv = rcp_approx(d), h = 0.5f * d, c2 = fmaf(-3.814697265625e-06f, d, c);
@@ -171,18 +172,19 @@ MADI_DEV void code_words(const float (&x)[16], float c, float d, uint32_t (&w)[2
     }
     if (!(least > -h && most < h)) {
         bool wrong = least < -h || most >= h;
-        if (!wrong) {                                        // r + d/2 + (x - c - t) < 0 only if r = -d/2
+        if (!wrong) {                                        // t - (n' - 1/2) d + (x - c - t) < 0 only if r = -d/2
 #pragma unroll
             for (int q = 0; q < 16; q += 2) {
-                float t0, t1, b0, b1, u0, u1, e0, e1, r0, r1;
+                float t0, t1, b0, b1, u0, u1, e0, e1, s0, s1;
                 add2(t0, t1, x[q], x[q + 1], -c, -c);
                 add2(b0, b1, t0, t1, -x[q], -x[q + 1]);
                 add2(u0, u1, t0, t1, -b0, -b1);
                 add2(u0, u1, x[q], x[q + 1], -u0, -u1);
                 add2(e0, e1, -c, -c, -b0, -b1);
                 add2(e0, e1, u0, u1, e0, e1);
-                fma2(r0, r1, z[q], z[q + 1], -d, -d, t0, t1);
-                wrong = wrong || (r0 + h) + e0 < 0.f || (r1 + h) + e1 < 0.f;
+                add2(s0, s1, -z[q], -z[q + 1], 0.5f, 0.5f);
+                fma2(s0, s1, s0, s1, d, d, t0, t1);
+                wrong = wrong || s0 + e0 < 0.f || s1 + e1 < 0.f;
             }
         }
         if (wrong) {

@@ -160,3 +160,39 @@ def test_store_of_the_smallest_numbers(madi):
     for kv in (0, 1):
         gz, gc, gd = R.unpack(c.data.cpu().numpy(), kv, len(x))
         assert np.array_equal(gc[0, 0], cc) and np.array_equal(gd[0, 0], dd) and np.array_equal(gz[0, 0], z)
+
+
+def test_store_beside_the_halves_of_a_step(madi):
+    """Elements on a half of a step and up to three places beside it, every code, for steps that are
+    powers of two and others, around zero and far from it: the definition's bytes."""
+    import torch
+    from madi_b200 import kv4
+    g = np.random.default_rng(11)
+    rows = []
+    for d in (2.0 ** -24, 3 * 2.0 ** -24, 2.0 ** -20, 0.25, 0.375, 1.0, 129 / 128, 2.0, 1024.0):
+        for c in (0.0, -0.0, 1.5 * d, -3 * d, 64 * d, 1000 * d):
+            c = float(np.float16(np.clip(c, -20000, 20000)))
+            for n in range(-7, 8):
+                for off in (None, -2, -1, 0, 1, 2):
+                    # on or beside the half below code n: one such element in each lane's sixteen, the others
+                    # on their values, or (off None) all of them within three places of one
+                    x = (c + g.integers(-8, 8, 64) * d).astype(np.float32)
+                    x[1], x[2] = c - 8 * d, c + 7 * d             # the range that gives c and d, nearly
+                    half = np.float32(c + (n - 0.5) * d).view(np.int32)
+                    if off is None:
+                        x[3:] = (half + g.integers(-3, 4, 61).astype(np.int32) * (half != 0)).view(np.float32)
+                    else:
+                        x[g.integers(3, 16)::16] = (half + np.int32(off)).view(np.float32)
+                    rows.append(np.where(np.abs(x) <= 57344, x, 0))
+    x = np.array(rows, np.float32)
+    for dt in (np.float32, np.float16):
+        y = x.astype(dt)
+        c4 = kv4.Cache.empty(1, 1, len(y))
+        Y = torch.from_numpy(y[None]).cuda()
+        kv4.store(c4, Y, Y)
+        z, cc, dd = R.quantise(y)
+        torch.cuda.synchronize()
+        for kv in (0, 1):
+            gz, gc, gd = R.unpack(c4.data.cpu().numpy(), kv, len(y))
+            assert np.array_equal(gc[0, 0], cc) and np.array_equal(gd[0, 0], dd)
+            assert np.array_equal(gz[0, 0], z), f"{(gz[0, 0] != z).sum()} codes differ"

@@ -389,7 +389,7 @@ typedef struct madi_kv4_rows {
 int madi_kv4_store(const madi_kv4 *c, const madi_kv4_rows *r, void *stream);
 
 /* The reverse: cache rows into r's rows, the value rounded once.  Rows past max_tok and rows
- * i >= n[s] of k and v are left as they were. */
+ * i >= n[s] of k and v are left as they were.  k's and v's rows do not overlap. */
 int madi_kv4_load(const madi_kv4 *c, const madi_kv4_rows *r, void *stream);
 
 /* Attention of `rows` query rows per slot over the cache: row i of slot s, head h:
@@ -400,7 +400,12 @@ int madi_kv4_load(const madi_kv4 *c, const madi_kv4_rows *r, void *stream);
  * never used, whatever they hold.  q, out: dtype (both MADI_F32 or both MADI_F16), element
  * (s, i, j) at s * slot + i * row, j < heads * 64, 16-byte aligned rows; out does not overlap
  * q.  heads: a multiple of kv_heads, at most 1024.  pos, lens, n: u32 [slots] on the device or
- * NULL; not both of pos and lens.  q must be finite.  Takes no scratch memory. */
+ * NULL; not both of pos and lens.  q must be finite, and below 2^100 in magnitude.  Takes no
+ * scratch memory.  f32 results are as near the exact ones as plain f32 arithmetic comes (some
+ * 2e-7 to 3e-6 in norm, by the spread of the scores).  f16 results are the exact ones rounded, or, from
+ * 17 or 32 query columns (rows x heads / kv_heads) per kv head on, by slots x kv_heads, of weights
+ * rounded to f16 (2.6e-4 in norm for 2.1e-4): a row's last bits can depend on how many rows and
+ * slots share its call. */
 typedef struct madi_kv4_query {
     const void *q;
     void *out;

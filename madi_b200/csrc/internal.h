@@ -164,7 +164,7 @@ cudaError_t launch_self_attn(float *out, const float *q, const void *kc, const v
 // ---- encoder self-attention on the tensor cores (flash_enc.cu); head_dim 64
 cudaError_t launch_flash_enc(const __half *q, const __half *k, const __half *v, int stride, __half *out,
                              int out_stride, int seq, int heads, int chunks, int *dev_err, cudaStream_t st);
-// ---- K/V cache in 4 bits (kv4.cu, kv4_attn.cu; format in kv4.cuh); head_dim 64
+// ---- K/V cache in 4 bits (kv4.cu, kv4_attn.cu, kv4_flash.cu; format in kv4.cuh); head_dim 64
 struct Kv4Args {
     uint8_t *data;                       // [slots][kv_heads][blocks of 64 tokens][4608]
     int slots, kv_heads, max_tok;

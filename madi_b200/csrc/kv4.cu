@@ -205,9 +205,10 @@ MADI_DEV void code_words(const float (&x)[16], float c, float d, uint32_t (&w)[2
     }
 }
 
-// Bound by its instructions and the latency of its loads: 24.8 us for 8 x 1500 f16 rows of 20 heads (78 MB,
-// 3.2 TB/s).  Six CTAs per SM (80 registers): with the 102 it would take 30.5 us, with 64, spilling, 30.8;
-// with CTAs of 256 threads and 64 rows 26.6.
+// Bound by its instructions and the latency of its loads: 23.0 us for 8 x 1500 f16 rows of 20 heads (79 MB,
+// 3.4 TB/s), 24.5 for f32 ones (140 MB, 5.7 TB/s).  Six CTAs per SM: 80 registers, of which two spill.  Measured at an
+// earlier state that took 24.8: 30.5 with the 102 registers it would take, 30.8 with 64; 26.6 with CTAs of 256
+// threads and 64 rows.
 // No pointer of these kernels is __restrict__: their memory is written while they are already resident (by the
 // kernel before them, until pdl_wait), so loads through the read-only path would be wrong.
 template <typename T>
@@ -305,7 +306,7 @@ MADI_DEV void st_values(__half *p, const Codes2 &u, __half2 cd, int j) {
     reinterpret_cast<uint4 *>(p)[j] = make_uint4(e[0], e[1], e[2], e[3]);
 }
 
-// Bound by its writes: 24.4 us for those rows as f32 (140 MB, 5.7 TB/s = 88 % of a copy's rate).
+// Bound by its writes: 24.2 us for those rows as f32 (140 MB, 5.8 TB/s = 88 % of a copy's rate).
 template <typename T>
 __global__ void __launch_bounds__(kThr) kv4_load_kernel(const uint8_t *data, long long slot_bytes, long long head_bytes,
                                                         int max_tok, T *k, T *v, long long slot_stride,
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(kThr) kv4_load_kernel(const uint8_t *data, lon
 
 long long head_bytes(const Kv4Args &a) { return (long long)((a.max_tok + kKv4Blk - 1) / kKv4Blk) * kKv4Block; }
 
-// Threads per CTA: `lanes` per row, at most 256.
+// Threads per CTA: `lanes` per row, at most kThr.
 int threads_for(int rows, int lanes) { return rows * lanes >= kThr ? kThr : (rows * lanes + 31) / 32 * 32; }
 
 template <typename T>

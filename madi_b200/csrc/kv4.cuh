@@ -1,4 +1,4 @@
-// kv4.cuh -- the 4-bit K/V cache format shared by its kernels (kv4.cu, kv4_attn.cu).
+// kv4.cuh -- the 4-bit K/V cache format shared by its kernels (kv4.cu, kv4_attn.cu, kv4_flash.cu).
 //
 // A group is the 64 elements of one (token, kv head), stored as 64 nibbles n' + 8 with
 // n' in -8..7 and two f16: value = c + d n'.  d has at most 8 significant bits, so d n'
@@ -20,6 +20,14 @@ constexpr int kKv4Blk = 64;                             // tokens per block
 constexpr int kKv4Codes = kKv4Blk * 32;                 // bytes of one block's K (or V) codes
 constexpr int kKv4Half = kKv4Codes + kKv4Blk * 4;       // codes + (c, d)
 constexpr int kKv4Block = 2 * kKv4Half;                 // 4608
+
+// 2^e for -126 <= e <= 127.
+MADI_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+MADI_DEV float max3f(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // Keys the query at row i of slot s attends to: rows 0 .. pos[s] + i, or 0 .. lens[s] - 1,
 // or the whole cache; never past max_tok.

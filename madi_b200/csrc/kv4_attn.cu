@@ -86,11 +86,6 @@ MADI_DEV uint32_t movm_trans(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-MADI_DEV float max3f(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 MADI_DEV uint32_t cluster_id_x() {
     uint32_t r;
     asm("mov.u32 %0, %%clusterid.x;" : "=r"(r));
@@ -155,15 +150,14 @@ MADI_DEV void ld16(const __half *p, float (&f)[16]) {
 }
 MADI_DEV void stf(float *p, float v) { *p = v; }
 MADI_DEV void stf(__half *p, float v) { *p = __float2half_rn(v); }
-// 2^e for -126 <= e <= 127.
-MADI_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // floor(log2 x) of a positive normal f32.
 MADI_DEV int ilog2f_(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
 
 // One warp's partial result for a column: running max (base 2), sum, and unnormalised output.
 constexpr int kPart = 2 + kKv4Hd;
 
-// NT groups of four query columns per CTA of W warps.
+// NT groups of four query columns per CTA of W warps.  115 to 185 registers; with four groups 255, and 8 to 60 bytes
+// (f32) or some 300 to 380 (f16) spilled.
 template <int NT, int W, typename T>
 __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(const Kv4AttnArgs a, long long slot_bytes,
                                                             long long head_bytes, int group, int ns, int stages) {
@@ -584,8 +578,11 @@ __global__ void __launch_bounds__(32 * W, NT > 1 ? 1 : 2) kv4_stream_kernel(cons
 }
 
 // f16 query columns (rows x query heads per kv head) from which the tensor-core tiles of kv4_flash.cu
-// are faster: 32, or with a (slot, kv head) per SM what no longer fits one tile here.  Measured (us, here
-// and there): 8 slots x 20 heads x 1500 keys 16 columns 24, 33; 17 42, 34; 32 42, 34; 16 x 20 x 448
+// run: 32, or with a (slot, kv head) per SM what no longer fits one tile here.  They round the weights to f16
+// where this form keeps 22 bits: 2.6e-4 in norm against the 2.1e-4 of a result rounded once, which is why
+// calls that fit one tile here stay here although the crossover of the times lies near.  The rule goes by the number of
+// pairs alone; with few pairs of long caches the tiles would be faster from some 20 columns.  Measured (us, here and
+// there): 8 slots x 20 heads x 1500 keys 16 columns 24, 33; 17 42, 34; 32 42, 34; 16 x 20 x 448
 // 20 columns 31, 24.  Fewer pairs: 1 x 20 x 1500 24 columns 11.0, 14.4; 1 x 20 x 448 32 columns 10.9, 11.3;
 // 4 x 8 x 16000 24 columns 59, 50, 4 x 8 x 1000 11.0, 16.3, 2 x 8 x 60000 20 columns 122, 148.
 constexpr int kFlashCols = 32;
@@ -625,10 +622,11 @@ cudaError_t launch_stream(const Kv4AttnArgs &a, long long tiles, int ns, cudaStr
 // short cache has to be cut up finely.  Measured (us): 8 slots x 20 heads x 1500 keys 8.1 as 3 CTAs of 4
 // (8.9 as 1 of 8, 10.3 as 6 of 4), 16 x 20 x 448 ragged 5.7 as 1 of 4 (6.2 as 1 of 8), 8 x 8 x 6000
 // 10.2 as 4 of 8 (10.5 as 8 of 4), 1 x 20 x 1500 4.3 as 6 of 4 (4.7 as 3 of 8), 4 x 8 x 65003 ragged
-// 28.9 as 16 of 8 (32.9 as 8 of 8).
+// 28.9 as 16 of 8 (32.9 as 8 of 8).  (f32 figures of choices not taken, here and below, from before the values' codes
+// became normal numbers, which adds 0 to 15 %: the chosen ones take 8.7, 6.0, 10.5 and 4.5 now.)
 // With more (slot, kv head, tile)s than that, a CTA's idle warps and its join only take room from the
 // next one: CTAs of two warps, of one for one or two blocks.  Measured with 4, 2 and 1 warps (us):
-// f32, 14 slots x 50 rows x 32 / 4 heads x 52 keys 45.6, 32.4, 28.0; 8 x 48 x 20 x 1500 46.6, 42.4, 71;
+// f32, 14 slots x 50 rows x 32 / 4 heads x 52 keys 45.6, 32.4, 28.0 (now 26.1); 8 x 48 x 20 x 1500 46.6, 42.4, 71;
 // 32 x 5 x 20 x 448 15.1, 10.9, 14.6; x 100 12.7, 9.5, 8.3; one
 // column group: 64 x 1 x 20 x 64 8.5, 6.9, 5.3; 40 x 1 x 20 x 1500 (two sets of warps an SM) 22.3, 25.6, 35.9.
 template <int NT, typename T>

@@ -107,12 +107,6 @@ MADI_DEV void tmem_ld2(uint32_t taddr, uint32_t &r0, uint32_t &r1) {
 MADI_DEV void tmem_st2(uint32_t taddr, uint32_t r0, uint32_t r1) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(r0), "r"(r1) : "memory");
 }
-MADI_DEV float max3f(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-MADI_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // 16-byte chunk c of row r of a [..][64] f16 tile in the SWIZZLE_128B layout.
 MADI_DEV uint4 *chunk(uint8_t *tile, int r, int c) {
@@ -503,7 +497,7 @@ __global__ void __launch_bounds__(FlashCfg<kX>::kThr, FlashCfg<kX>::kPerSm)
             // The cluster's partials: this CTA's rows into the ring's place (its products are
             // done), then every CTA joins its share of the rows from all of them.
             named_bar_sync(0, kThr);
-            float *part = reinterpret_cast<float *>(ring);   // [256][kPartW]
+            float *part = reinterpret_cast<float *>(ring);   // [kX * kQT][kPartW]
             float *p = part + (x * kQT + row) * kPartW;
             const bool have = alive && n > 0;
             p[kKv4Hd] = have ? m : -CUDART_INF_F;
@@ -602,9 +596,9 @@ cudaError_t launch_flash(const Kv4AttnArgs &a, cudaStream_t st) {
 
 }  // namespace
 
-// One query tile per CTA where the columns fit one (8 slots x 20 heads x 1500 keys: 64 columns 34 us, with
-// two 43; 128: 36, 44), else two, which share the keys they unpack (2 x 1024 rows x 32 heads, 16640 keys:
-// 349 us, with one 363).
+// One query tile per CTA where the columns fit one (8 slots x 20 heads x 1500 keys: 64 columns 35 us, with
+// two 43; 128: 36, 44; 128 registers, some 60 bytes spilled, for two CTAs an SM), else two, which share the keys they unpack (2 x 1024 rows x 32 heads, 16640 keys:
+// 352 us; 349 and 363 with one at an earlier state).
 cudaError_t launch_kv4_flash(const Kv4AttnArgs &a, cudaStream_t st) {
     return (long long)a.rows * (a.heads / a.c.kv_heads) <= kQT ? launch_flash<1>(a, st) : launch_flash<2>(a, st);
 }

@@ -31,7 +31,10 @@ rows); an all-gather of the per-row (max, index, exp sum) parts; and the merge
 K/V caches in 4 bits (kv4_cache=True): 36 bytes per token and head instead of 256 (self) and 128
 (cross), K and V each.  The QKV projection leaves the new rows in a one-row buffer, kv4.store
 quantises them into the cache at the slot's position, and both attentions read the 4-bit
-caches (kv4.attn); the cross K / V are quantised once per audio chunk.
+caches (kv4.attn); the cross K / V are quantised once per audio chunk, from f16 projections whose
+buffers (one layer's, 61 MB at 8 slots) stay with the decoder.  That pays from several slots on:
+a captured token step takes 249 us for 271 at 8 slots, 317 for 358 at 15, but 240 for 216 at one
+(one more launch a layer, and little to read).
 """
 from dataclasses import dataclass
 from typing import Callable, List, Optional, Tuple
@@ -134,7 +137,8 @@ class Decoder:
         split: (world, rank) for the column-split vocab head (see the module
         docstring); exchange(out, inp): all-gather of inp from every rank into out,
         rank-major (default: torch.distributed.all_gather_into_tensor).
-        kv4_cache: keep the self and cross K / V in 4 bits (see the module docstring)."""
+        kv4_cache: keep the self and cross K / V in 4 bits (see the module docstring: slower at one
+        slot, and the results differ by what 16 values an element leave off, see kv4)."""
         if not 1 <= slots <= 16:
             raise ValueError("1..16 token slots")
         if split is not None and not (split[0] >= 1 and 0 <= split[1] < split[0]):
@@ -202,7 +206,8 @@ class Decoder:
 
     def set_encoder(self, enc_states: torch.Tensor, stream=None):
         """Cross K / V of every layer from the encoder states f16 [slots][1500][1280]
-        (the tcgen05 GEMM, once per audio chunk); kept f16 as the reference's decoder does.
+        (the tcgen05 GEMM, once per audio chunk); kept f16 as the reference's decoder does, or
+        quantised to 4 bits (kv4_cache).
         The K / V buffers are reused while their shape holds, so a captured token step
         stays valid across audio chunks."""
         S, T, _ = enc_states.shape
@@ -234,8 +239,9 @@ class Decoder:
         tok[:, 0] = seed_token
         conf.zero_()
         pos.zero_()
-        for c in self.kc + self.vc:
-            c.zero_()
+        if not self.kv4_cache:                               # (then: one row, written before it is read)
+            for c in self.kc + self.vc:
+                c.zero_()
 
     def step(self, sample_begin: int = 1, no_repeat_ngram: int = 0, stream=None, suppress=None):
         """One greedy token for every slot; all state on the device.  suppress: device

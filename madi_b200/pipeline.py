@@ -59,7 +59,7 @@ class Transcriber:
         all_gather_into_tensor), "p2p" (madi_b200.p2p.PeerExchange: one kernel storing
         into the peers' memory over NVLink; ranks on distinct GPUs), or "auto" (the
         default: p2p when the ranks sit on distinct GPUs, else nccl).
-        kv4_cache: the decoders keep their K / V caches in 4 bits (decoder.Decoder)."""
+        kv4_cache: the decoders keep their K / V caches in 4 bits (decoder.Decoder; slower at one slot)."""
         if tokens < 1 or tokens + 1 > dec.MAX_TOK:
             raise ValueError(f"1..{dec.MAX_TOK - 1} tokens per chunk")
         self.encoder = enc.Encoder(enc_layers, seed, device)

@@ -138,6 +138,26 @@ def test_f32_values_beside_a_large_one_of_no_weight(madi, rows, heads, kv_heads,
     assert err <= F32_SUMS + 5 * 2.0 ** -24 * 6, f"{err:.2e}"
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 2, 1), (7, 2, 2), (20, 1, 1)])
+@pytest.mark.parametrize("scale", [1e-38, 1e-20, 2.0 ** 20, 2.0 ** 60, 2.0 ** 97])
+def test_f32_query_magnitudes(madi, rows, heads, kv_heads, scale):
+    """From the smallest normal queries (a flat softmax) to nearly the largest the interface takes: there the
+    key of the largest score alone counts, if its lead is more than the scores' rounding, 2^-18 of the largest
+    magnitudes (a few hundred f32 units), which all rows' is here."""
+    import torch
+    rn = _gen(rows)
+    M = 200
+    q = rn(2, rows, heads * 64).clamp(-4, 4) * scale
+    c, k, v, _ = _stored(rn(2, M, kv_heads * 64), rn(2, M, kv_heads * 64), kv_heads)
+    if scale > 1:
+        z = _split(q, kv_heads) @ k.transpose(-1, -2)
+        top = z.topk(2, dim=-1).values
+        lead = (top[..., 0] - top[..., 1]) / (_split(q, kv_heads).abs().sum(-1) * 4)
+        assert lead.min().item() > 2.0 ** -18, "another seed"
+    err = _norm_error(q, c, k, v, heads, kv_heads)
+    assert err <= F32_SUMS + 5 * 2.0 ** -24 * 6, f"{err:.2e}"
+
+
 def test_store_of_the_smallest_numbers(madi):
     """Groups of a few 2^-149 on one side or both, whose step has to be 2^-24 and not 0: the same bytes
     as the format's definition gives."""
